@@ -51,6 +51,7 @@ extern "C" {
 
 #define TVAE_F32 0
 #define TVAE_BF16 1
+#define TVAE_F16 3     /* storage type of the rows of the 8-bit cache and of logits; no GEMM arithmetic */
 #define TVAE_F32X3 2   /* fp32-accurate GEMM from six bf16 MFMAs on exact 3-way bf16 splits of the operands */
 
 /* gemm flags */
@@ -407,6 +408,66 @@ int tvae_encode_smiles(const char* text, const int64_t* offsets, int64_t n, cons
                        int n_threads, int64_t* bad_row, int* bad_code);
 int tvae_gather_batch(const uint8_t* ids, int64_t ld_ids, const float* props, const int64_t* index,
                       int64_t first, int64_t n_rows, int B, int L, float* out, int ldo, void* stream);
+
+/*
+ * A key/value cache in 8 bits (no counterpart in the reference, which keeps no cache: greedy_decode recomputes every position,
+ * transvae/trans_models.py:418-434).  Four arrays hold a pool of n_pages pages of `page` tokens (a power of two, 16 .. 256):
+ *   kc, vc (n_pages, h, page, dk)  e4m3 codes, one byte each (dk 32, 64, 128 or 256)
+ *   ke, ve (n_pages, h)            exponents, bias 127, in [27, 246]: value = code * 2^(exponent - 127)
+ * Sequence b keeps its tokens i * page .. (i + 1) * page - 1 in page table[b * per_seq + i], or in page b * per_seq + i when
+ * table is NULL (then n * per_seq <= n_pages).  A table entry outside [0, n_pages) is no page: what would be stored there is
+ * dropped, what would be read is absent.  Two sequences may share a page that both only read.
+ * dtype (TVAE_F32, TVAE_BF16, TVAE_F16) is the type of k, v, q, o; their innermost dimension is dense and rows are 16-byte
+ * aligned; ld*b, ld*t (or ld*i), ld*h are the strides in elements of sequence, token and head.
+ *
+ *   store: rows t < min(T, count[b]) (count NULL: T) of k, v (n, T, h, dk) become tokens start[b] + t (start NULL: start0 + t).
+ *     Tokens past the last page are dropped, a negative start stores nothing.  The exponent of a (page, head) is the smallest e
+ *     with |x| 2^-e <= 448 over the page's new rows; where rows stand in front of them in the page it is no smaller than the
+ *     page's old one, and when it grows those rows are rounded again to the new scale.  What stands behind the new rows in
+ *     the page is left as it is and counts as dead.  Infinities and NaN are stored as NaN and do not count for the exponent.
+ *     Pages that one call stores to must be different for every sequence.
+ *   load: k, v (n, T, h, dk), contiguous: tokens start[b] + t; zeros where t >= count[b] or where there is no such token.
+ *   attn: o = softmax(scale q k^T) v of Lq query tokens, h * G query heads (head i attends key head i / G) over tokens
+ *     j < lens[b] (lens NULL: len0), with causal != 0 only j < lens[b] - (Lq - 1 - i) for query token i; key_mask (n, ld_mask)
+ *     or NULL: only j < mask_w with a non-zero byte.  A query that sees no key gets zeros (unlike tvae_decode_attn, whose
+ *     -1e9 fill lets it attend uniformly).  What stands in masked or dead places never matters, NaN included.
+ *     splits: the tokens are cut into that many parts (1 .. 1024), joined by a second launch over the workspace
+ *     ws of n * Lq * h * G * splits * (dk + 2) floats (splits 1: NULL).
+ */
+int tvae_kv8_store(const void* k, int64_t ldkb, int64_t ldkt, int64_t ldkh, const void* v, int64_t ldvb, int64_t ldvt,
+                   int64_t ldvh, int dtype, uint8_t* kc, uint8_t* vc, uint8_t* ke, uint8_t* ve, int n_pages,
+                   const int32_t* table, int per_seq, const int32_t* start, int start0, const int32_t* count, int n, int T,
+                   int h, int dk, int page, void* stream);
+int tvae_kv8_load(const uint8_t* kc, const uint8_t* vc, const uint8_t* ke, const uint8_t* ve, int n_pages,
+                  const int32_t* table, int per_seq, const int32_t* start, int start0, const int32_t* count, void* k, void* v,
+                  int dtype, int n, int T, int h, int dk, int page, void* stream);
+int tvae_kv8_attn(const void* q, int64_t ldqb, int64_t ldqi, int64_t ldqh, void* o, int64_t ldob, int64_t ldoi, int64_t ldoh,
+                  int dtype, const uint8_t* kc, const uint8_t* vc, const uint8_t* ke, const uint8_t* ve, int n_pages,
+                  const int32_t* table, int per_seq, const int32_t* lens, int len0, const uint8_t* key_mask, int64_t ld_mask,
+                  int mask_w, int causal, int n, int h, int G, int Lq, int dk, int page, float scale, int splits, float* ws,
+                  void* stream);
+
+/*
+ * Log probabilities of given tokens, entropies and the `top` (0 .. 64, <= V) most likely classes of rows of logits (no
+ * counterpart in the reference, whose losses give weighted means only, transvae/loss.py:8-38).  Row r: logits + r * ld, V
+ * values of dtype TVAE_F32, TVAE_BF16 or TVAE_F16, any alignment; class y = tokens[r * ld_tok] - tok_sub (tokens NULL or y
+ * outside [0, V): no token, logp 0).  With M = max x, L = ln sum exp(x - M):
+ *   logp[r * ld_logp] = x_y - M - L ; entropy[r * ld_ent] = L - sum exp(x - M) (x - M) / e^L ; stat (rows, 2) = {M, L}
+ *   top_ids, top_logp (rows, top): by descending logit, then ascending class (NaN above +inf)
+ * A row of -inf only: logp and top_logp -inf, entropy 0.  A NaN or +inf makes the row's values NaN.
+ * segs (1 .. 1024): rows are cut into that many parts, joined by a second launch over ws, rows * segs * (3 + 2 top) floats
+ * (segs 1: NULL).
+ *   bwd: dx (rows, V) contiguous, of the logits' type, from the forward's stat, entropy and top_ids and the gradients
+ *   g_logp (rows), g_entropy (rows), g_top (rows, top), each of which may be NULL; every element of dx is written:
+ *   dx_j = g_logp (d_jy - p_j) - g_entropy p_j (ln p_j + H) + sum_t g_top_t (d_{j, top_t} - p_j); 0 where the logit is -inf.
+ */
+int tvae_token_logp(const void* logits, int64_t ld, int dtype, const int64_t* tokens, int64_t ld_tok, int64_t tok_sub, int64_t rows,
+                    int64_t V, int top, float* logp, int64_t ld_logp, float* entropy, int64_t ld_ent, float* stat, float* top_logp,
+                    int64_t* top_ids, int segs, float* ws, void* stream);
+int tvae_token_logp_bwd(const void* logits, int64_t ld, int dtype, const int64_t* tokens, int64_t ld_tok, int64_t tok_sub,
+                        int64_t rows, int64_t V, int top, const float* stat, const float* entropy, int64_t ld_ent,
+                        const int64_t* top_ids, const float* g_logp, const float* g_entropy, const float* g_top, void* dx,
+                        void* stream);
 
 /* bump the dropout step counter: rng[1] += 1 (one tiny launch per train step, graph-safe) */
 int tvae_rng_advance(uint32_t* rng, void* stream);

@@ -13,7 +13,7 @@ import torch  # noqa: F401  -- FIRST: torch bundles its own libamdhip64; loading
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TVAE_LIB_PATH") or os.path.join(_HERE, "lib", "libtvae_hip.so")   # override: kernel experiments
 
-F32, BF16, F32X3 = 0, 1, 2
+F32, BF16, F32X3, F16 = 0, 1, 2, 3
 GEMM_RELU, GEMM_ACCUM, GEMM_A_KMAJOR, GEMM_B_KMAJOR, GEMM_SPLITK, GEMM_A_DROPMASK, GEMM_RELUMASK = 1, 2, 4, 8, 16, 32, 64
 GEMM_B_SPLIT3 = 128
 GEMM_B_BF16 = 256
@@ -62,6 +62,13 @@ SIGNATURES = {
     "tvae_residual_dropout": [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _u, _f, _vp],
     "tvae_rng_advance": [_vp, _vp],
     "tvae_encode_smiles": [_vp, _vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i, _vp, _vp],
+    "tvae_token_logp": [_vp, _i64, _i, _vp, _i64, _i64, _i64, _i64, _i, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _vp],
+    "tvae_token_logp_bwd": [_vp, _i64, _i, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+    "tvae_kv8_store": [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp,
+                       _i, _i, _i, _i, _i, _vp],
+    "tvae_kv8_load": [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    "tvae_kv8_attn": [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i, _vp, _i64,
+                      _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _vp],
     "tvae_gather_batch": [_vp, _i64, _vp, _vp, _i64, _i64, _i, _i, _vp, _i, _vp],
 }
 

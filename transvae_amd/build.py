@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libtvae_hip.so")
-SOURCES = ["gemm.hip", "gemm3.hip", "gemm3_dma.hip", "gemm_dma.hip", "gemm_wide.hip", "rowops.hip", "attention.hip", "lossopt.hip", "dataprep.hip", "gru.hip"]
+SOURCES = ["gemm.hip", "gemm3.hip", "gemm3_dma.hip", "gemm_dma.hip", "gemm_wide.hip", "rowops.hip", "attention.hip", "lossopt.hip", "dataprep.hip", "gru.hip", "kv8.hip", "score.hip"]
 # no packed fp32 instructions (v_pk_add / mul / fma_f32): hipcc -O3 forms them from ordinary float code, and some of their forms
 # have given wrong results on this hardware now and then.  The host pass does not know the feature and warns: harmless.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",

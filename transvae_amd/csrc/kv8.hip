@@ -1,0 +1,540 @@
+// Keys and values held in 8 bits: store (quantise rows as they are written), load (read them back) and attention over them.
+//
+// A cache is a pool of pages.  One page holds `page` tokens of every head: codes (n_pages, h, page, dk), one byte each, in
+// e4m3 (1 sign, 4 exponent, 3 mantissa bits, largest 448, no infinity), and one exponent byte per (page, head), bias 127:
+//     value = code * 2^(exponent - 127).
+// Why a power of two: e4m3 is itself floating point, so a finer scale would not add precision inside its normal range (2^-6 ..
+// 448), while a power of two makes scaling, un-scaling and re-scaling exact: a code is ONE rounding of the value it was made
+// from, and pulling the rows of a page down to a larger exponent only rounds what drops into the subnormals.
+// The exponent is the smallest with amax * 2^-e <= 448, held to [-100, 119] so that no value of a cache can overflow fp32.
+#include "common.h"
+
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+
+namespace {
+
+constexpr int E_BIAS = 127, E_MIN = 27, E_MAX = 246;
+constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;              // of 256 threads: a grid counts its threads in 32 bits
+
+struct F16 { _Float16 v; };
+struct B16 { uint16_t v; };
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static __device__ inline void load4(const float* p, float (&x)[4]) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+  }
+  static __device__ inline void put(float* p, float x) { *p = x; }
+};
+template <> struct Elem<B16> {
+  static __device__ inline void load4(const B16* p, float (&x)[4]) {
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(t.x << 16); x[1] = __uint_as_float(t.x & 0xFFFF0000u);
+    x[2] = __uint_as_float(t.y << 16); x[3] = __uint_as_float(t.y & 0xFFFF0000u);
+  }
+  static __device__ inline uint16_t cvt(float x) {         // round to nearest even; NaN stays NaN
+    const uint32_t u = __float_as_uint(x);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40);
+    return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+  }
+  static __device__ inline void put(B16* p, float x) { p->v = cvt(x); }
+};
+template <> struct Elem<F16> {
+  static __device__ inline void load4(const F16* p, float (&x)[4]) {
+    _Float16 h[4];
+    *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)h[i];
+  }
+  static __device__ inline void put(F16* p, float x) { p->v = (_Float16)x; }
+};
+
+__device__ inline float exp_scale(int e) { return __uint_as_float((uint32_t)e << 23); }          // 2^(e - 127)
+__device__ inline float inv_scale(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }  // 2^(127 - e)
+
+// stored exponent for a largest magnitude (448 = 1.75 * 2^8: a mantissa above 1.75 carries into the exponent)
+__device__ inline int need_exp(float amax) {
+  const int e = (int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 8;
+  return e < E_MIN ? E_MIN : e > E_MAX ? E_MAX : e;
+}
+__device__ inline float finite_abs(float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+  return u < 0x7F800000u ? __uint_as_float(u) : 0.f;
+}
+// e4m3 operand of a value: scaled and clamped (the largest exponent cannot hold every float), non-finite -> NaN (the format
+// has no infinity, and a saturated one would read back as an ordinary number)
+__device__ inline float to_range(float x, float inv) {
+  const float y = fminf(fmaxf(x * inv, -448.f), 448.f);
+  return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u ? __uint_as_float(0x7FC00000u) : y;
+}
+__device__ inline uint32_t pack4(const float (&y)[4]) {
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  return w;
+}
+__device__ inline void unpack4(uint32_t w, float (&x)[4]) {
+  const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+}
+
+// where a sequence's pages are
+struct Pages {
+  const int32_t* table;      // (n, per_seq) page ids, or NULL: page b * per_seq + i
+  int per_seq, n_pages;
+  __device__ inline int at(int b, int slot) const {
+    const int p = table ? table[(size_t)b * per_seq + slot] : b * per_seq + slot;
+    return p >= 0 && p < n_pages ? p : -1;                   // -1: no such page, nothing is read or written
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ store
+struct StoreArgs {
+  const void* src[2];
+  int64_t ldb[2], ldt[2], ldh[2];
+  uint8_t* codes[2];
+  uint8_t* exps[2];
+  Pages pages;
+  const int32_t* start;
+  const int32_t* count;
+  int start0, n, T, h, dk, page, slots;
+};
+
+// One wave per (sequence, touched page, head, K or V): the largest magnitude of the new rows, the page's exponent, then the
+// codes.  Rows in front of the new ones are only rewritten when the exponent grows.
+template <typename T>
+__global__ __launch_bounds__(256) void kv8_store_kernel(StoreArgs a) {
+  const int lane = threadIdx.x & 63;
+  int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int side = (int)(unit & 1);
+  unit >>= 1;
+  const int head = (int)(unit % a.h);
+  unit /= a.h;
+  const int slot = (int)(unit % a.slots), b = (int)(unit / a.slots);
+  if (b >= a.n) return;
+  const int64_t beg = a.start ? a.start[b] : a.start0;
+  int cnt = a.count ? a.count[b] : a.T;
+  cnt = cnt < a.T ? cnt : a.T;
+  if (beg < 0 || cnt <= 0) return;
+  const int64_t pslot = beg / a.page + slot;
+  if (pslot >= a.pages.per_seq) return;
+  const int64_t p0 = pslot * a.page;                                     // first position of the page
+  const int r0 = (int)(beg > p0 ? beg - p0 : 0);                         // rows [r0, r1) of the page are new
+  const int64_t left = beg + cnt - p0;
+  const int r1 = (int)(left < a.page ? left : a.page);
+  if (r0 >= r1) return;
+  const int id = a.pages.at(b, (int)pslot);
+  if (id < 0) return;
+  const int lpr = a.dk >> 2, sub = lane % lpr, rg = lane / lpr, rpi = 64 / lpr;   // lanes per row, 4 values each
+  const T* src = reinterpret_cast<const T*>(a.src[side]) + (int64_t)b * a.ldb[side] + (int64_t)head * a.ldh[side] + 4 * sub;
+  const int64_t t0 = p0 - beg;
+  float amax = 0.f;
+  for (int r = r0 + rg; r < r1; r += rpi) {
+    float x[4];
+    Elem<T>::load4(src + (t0 + r) * a.ldt[side], x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, finite_abs(x[i]));
+  }
+  amax = wave_max(amax);
+  uint8_t* ep = a.exps[side] + (size_t)id * a.h + head;
+  uint8_t* dst = a.codes[side] + ((size_t)id * a.h + head) * a.page * a.dk + 4 * sub;
+  int e = need_exp(amax);
+  if (r0 > 0) {
+    const int old = *ep;
+    if (old >= e) {
+      e = old < E_MAX ? old : E_MAX;
+    } else {
+      int d = old - e;
+      d = d > -40 ? d : -40;                                            // beyond that everything rounds to zero
+      const float f = exp_scale(E_BIAS + d);
+      for (int r = rg; r < r0; r += rpi) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(dst + (size_t)r * a.dk);
+        float x[4];
+        unpack4(*w, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= f;
+        *w = pack4(x);
+      }
+    }
+  }
+  const float inv = inv_scale(e);
+  for (int r = r0 + rg; r < r1; r += rpi) {
+    float x[4];
+    Elem<T>::load4(src + (t0 + r) * a.ldt[side], x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = to_range(x[i], inv);
+    *reinterpret_cast<uint32_t*>(dst + (size_t)r * a.dk) = pack4(x);
+  }
+  if (lane == 0) *ep = (uint8_t)e;
+}
+
+// ------------------------------------------------------------------------------------------------ load
+struct LoadArgs {
+  const uint8_t* codes[2];
+  const uint8_t* exps[2];
+  void* out[2];
+  Pages pages;
+  const int32_t* start;
+  const int32_t* count;
+  int start0, n, T, h, dk, page;
+};
+
+// One thread per 4 values.
+template <typename T>
+__global__ __launch_bounds__(256) void kv8_load_kernel(LoadArgs a) {
+  const int side = blockIdx.y;
+  const int lpr = a.dk >> 2;
+  const int64_t total = (int64_t)a.n * a.h * a.T * lpr;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int sub = (int)(i % lpr);
+  i /= lpr;
+  const int t = (int)(i % a.T);
+  i /= a.T;
+  const int head = (int)(i % a.h), b = (int)(i / a.h);
+  const int64_t beg = a.start ? a.start[b] : a.start0;
+  int cnt = a.count ? a.count[b] : a.T;
+  const int64_t pos = beg + t;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (t < cnt && pos >= 0 && pos < (int64_t)a.pages.per_seq * a.page) {
+    const int id = a.pages.at(b, (int)(pos / a.page));
+    if (id >= 0) {
+      const size_t ph = (size_t)id * a.h + head;
+      unpack4(*reinterpret_cast<const uint32_t*>(a.codes[side] + (ph * a.page + pos % a.page) * a.dk + 4 * sub), x);
+      const float s = exp_scale(a.exps[side][ph]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] *= s;
+    }
+  }
+  T* o = reinterpret_cast<T*>(a.out[side]) + (((int64_t)b * a.T + t) * a.h + head) * a.dk + 4 * sub;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) Elem<T>::put(o + e, x[e]);
+}
+
+// ------------------------------------------------------------------------------------------------ attend
+struct AttnArgs {
+  const void* q;
+  void* o;
+  int64_t ldqb, ldqi, ldqh, ldob, ldoi, ldoh;
+  const uint8_t* codes[2];
+  const uint8_t* exps[2];
+  Pages pages;
+  const int32_t* lens;
+  const uint8_t* mask;
+  float* ws;                 // splits > 1: (rows, splits, dk) sums, then (rows, splits, 2) {max, sum of weights}
+  int64_t rows, ld_mask;
+  int mask_w, len0, causal, n, h, G, Lq, page, splits, chunk;
+  float scale;               // of the scores, times log2(e)
+};
+
+template <int CTRL> __device__ inline float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+// sum over groups of N neighbouring lanes (every lane of a group gets it): quad permutes, then mirrors of 8 and of 16
+template <int N> __device__ inline float group_sum(float x) {
+  if (N >= 2) x += dpp<0xB1>(x);
+  if (N >= 4) x += dpp<0x4E>(x);
+  if (N >= 8) x += dpp<0x141>(x);
+  if (N >= 16) x += dpp<0x140>(x);
+  return x;
+}
+
+__device__ inline int seq_len(const AttnArgs& a, int b) {
+  int64_t len = a.lens ? a.lens[b] : a.len0;
+  const int64_t cap = (int64_t)a.pages.per_seq * a.page;
+  len = len < cap ? len : cap;
+  return (int)(len > 0 ? len : 0);
+}
+
+// One query row at a time, without matrix instructions: DK / 16 lanes share a key (16 codes each), 64 / (DK / 16) keys an
+// instruction, four such groups of keys in flight.  Every lane group keeps a softmax of its own (running maximum, sum, its 16
+// dimensions); they meet once at the end.  Masked keys are not read.
+template <typename T, int DK, int KW>
+__global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
+  constexpr int LPK = DK / 16, NK = 64 / LPK, U = 4, KPI = NK * U;
+  __shared__ float sm[4][DK + 2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = KW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  const int kw = KW == 1 ? 0 : wave;
+  if (row >= a.rows) return;                                            // KW == 4: one row per block, uniform
+  const int g = (int)(row % a.G);
+  int64_t rest = row / a.G;
+  const int i = (int)(rest % a.Lq);
+  rest /= a.Lq;
+  const int head = (int)(rest % a.h), b = (int)(rest / a.h);
+  const int part = lane % LPK, kg = lane / LPK;
+  int end = seq_len(a, b) - (a.causal ? a.Lq - 1 - i : 0);
+  const int split = blockIdx.y;
+  const int64_t beg = (int64_t)split * a.chunk;
+  if (end > beg + a.chunk) end = (int)(beg + a.chunk);
+  float qr[16];
+  const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)b * a.ldqb + (int64_t)i * a.ldqi + (int64_t)(head * a.G + g) * a.ldqh + 16 * part;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float x[4];
+    Elem<T>::load4(q + 4 * c, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qr[4 * c + e] = x[e];
+  }
+  float m = -INFINITY, l = 0.f, o[16];
+#pragma unroll
+  for (int d = 0; d < 16; ++d) o[d] = 0.f;
+  for (int64_t j0 = beg + (int64_t)kw * KPI; j0 < end; j0 += (int64_t)KW * KPI) {
+    uint4 kc[U], vc[U];
+    float ks[U], vs[U], s[U];
+    bool vis[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t j = j0 + u * NK + kg;
+      bool see = j < end;
+      if (see && a.mask) see = j < a.mask_w && a.mask[(int64_t)b * a.ld_mask + j] != 0;
+      int id = -1;
+      if (see) id = a.pages.at(b, (int)(j / a.page));
+      see = id >= 0;
+      kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
+      ks[u] = vs[u] = 0.f;
+      if (see) {
+        const size_t ph = (size_t)id * a.h + head;
+        const size_t off = (ph * a.page + (int)(j % a.page)) * DK + 16 * part;
+        kc[u] = *reinterpret_cast<const uint4*>(a.codes[0] + off);
+        vc[u] = *reinterpret_cast<const uint4*>(a.codes[1] + off);
+        ks[u] = exp_scale(a.exps[0][ph]);
+        vs[u] = exp_scale(a.exps[1][ph]);
+      }
+      vis[u] = see;
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t w[4] = {kc[u].x, kc[u].y, kc[u].z, kc[u].w};
+      float acc = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float x[4];
+        unpack4(w[c], x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = fmaf(x[e], qr[4 * c + e], acc);
+      }
+      acc = group_sum<LPK>(acc) * (ks[u] * a.scale);
+      s[u] = vis[u] ? acc : -INFINITY;
+      mn = fmaxf(mn, s[u]);
+    }
+    const float ms = mn == -INFINITY ? 0.f : mn;                        // nothing seen so far: every weight is 0
+    const float al = __builtin_amdgcn_exp2f(m - ms);
+    m = mn;
+    l *= al;
+#pragma unroll
+    for (int d = 0; d < 16; ++d) o[d] *= al;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float p = __builtin_amdgcn_exp2f(s[u] - ms);
+      l += p;
+      const float pv = p * vs[u];
+      const uint32_t w[4] = {vc[u].x, vc[u].y, vc[u].z, vc[u].w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float x[4];
+        unpack4(w[c], x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[4 * c + e] = fmaf(x[e], pv, o[4 * c + e]);
+      }
+    }
+  }
+  // the lane groups meet
+  float M = m;
+#pragma unroll
+  for (int d = LPK; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  const float f = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+  l *= f;
+#pragma unroll
+  for (int d = 0; d < 16; ++d) o[d] *= f;
+#pragma unroll
+  for (int d = LPK; d < 64; d <<= 1) {
+    l += __shfl_xor(l, d, 64);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[c] += __shfl_xor(o[c], d, 64);
+  }
+  if (KW > 1) {
+    if (kg == 0) {
+#pragma unroll
+      for (int c = 0; c < 16; ++c) sm[wave][16 * part + c] = o[c];
+      if (part == 0) { sm[wave][DK] = M; sm[wave][DK + 1] = l; }
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    float MM = -INFINITY;
+    for (int w = 0; w < KW; ++w) MM = fmaxf(MM, sm[w][DK]);
+    const float z = MM == -INFINITY ? 0.f : MM;
+    l = 0.f;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) o[c] = 0.f;
+    for (int w = 0; w < KW; ++w) {
+      const float r = __builtin_amdgcn_exp2f(sm[w][DK] - z);
+      l += r * sm[w][DK + 1];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) o[c] += r * sm[w][16 * part + c];
+    }
+    M = MM;
+  }
+  if (kg != 0) return;
+  if (a.splits > 1) {
+    float* dst = a.ws + (row * a.splits + split) * DK + 16 * part;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) dst[c] = o[c];
+    if (part == 0) {
+      float* ml = a.ws + a.rows * a.splits * DK + (row * a.splits + split) * 2;
+      ml[0] = M;
+      ml[1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;                           // no visible key: zeros
+  T* dst = reinterpret_cast<T*>(a.o) + (int64_t)b * a.ldob + (int64_t)i * a.ldoi + (int64_t)(head * a.G + g) * a.ldoh + 16 * part;
+#pragma unroll
+  for (int c = 0; c < 16; ++c) Elem<T>::put(dst + c, o[c] * inv);
+}
+
+// joins the parts of a split row: one wave a row
+template <typename T>
+__global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a, int dk) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const int g = (int)(row % a.G);
+  int64_t rest = row / a.G;
+  const int i = (int)(rest % a.Lq);
+  rest /= a.Lq;
+  const int head = (int)(rest % a.h), b = (int)(rest / a.h);
+  const float* ml = a.ws + a.rows * a.splits * dk + row * a.splits * 2;
+  const float* part = a.ws + row * a.splits * dk;
+  float M = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) M = fmaxf(M, ml[2 * s]);
+  M = wave_max(M);
+  const float z = M == -INFINITY ? 0.f : M;
+  float l = 0.f;
+  for (int s = lane; s < a.splits; s += 64) l += __builtin_amdgcn_exp2f(ml[2 * s] - z) * ml[2 * s + 1];
+  l = wave_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* dst = reinterpret_cast<T*>(a.o) + (int64_t)b * a.ldob + (int64_t)i * a.ldoi + (int64_t)(head * a.G + g) * a.ldoh;
+  for (int d = lane; d < dk; d += 64) {
+    float acc = 0.f;
+    for (int s = 0; s < a.splits; ++s) acc += __builtin_amdgcn_exp2f(ml[2 * s] - z) * part[(int64_t)s * dk + d];
+    Elem<T>::put(dst + d, acc * inv);
+  }
+}
+
+bool page_ok(int page) { return page >= 16 && page <= 256 && (page & (page - 1)) == 0; }
+bool dk_ok(int dk) { return dk == 32 || dk == 64 || dk == 128 || dk == 256; }
+int type_bytes(int dtype) { return dtype == TVAE_F32 ? 4 : dtype == TVAE_BF16 || dtype == TVAE_F16 ? 2 : 0; }
+
+// the checks that the three entry points share
+int check_cache(const char* who, const uint8_t* kc, const uint8_t* vc, const uint8_t* ke, const uint8_t* ve, int n_pages,
+                const int32_t* table, int per_seq, int n, int h, int dk, int page, int dtype) {
+  TVAE_CHECK(kc && vc && ke && ve, TVAE_E_NULL, "%s: null cache pointer", who);
+  TVAE_CHECK(type_bytes(dtype), TVAE_E_DTYPE, "%s: dtype %d is not TVAE_F32, TVAE_BF16 or TVAE_F16", who, dtype);
+  TVAE_CHECK(n >= 0 && h > 0 && dk_ok(dk) && page_ok(page), TVAE_E_SHAPE,
+             "%s: need n >= 0, h >= 1, dk in {32, 64, 128, 256}, page a power of two in [16, 256] (n=%d h=%d dk=%d page=%d)", who, n, h, dk, page);
+  TVAE_CHECK(n_pages >= 0 && per_seq >= 1 && (int64_t)per_seq * page <= INT32_MAX, TVAE_E_SHAPE,
+             "%s: bad page counts (n_pages=%d, %d a sequence of %d tokens)", who, n_pages, per_seq, page);
+  TVAE_CHECK(table || (int64_t)n * per_seq <= n_pages, TVAE_E_SHAPE, "%s: %d sequences of %d pages do not fit %d pages", who, n, per_seq, n_pages);
+  TVAE_CHECK(aligned16(kc) && aligned16(vc), TVAE_E_SHAPE, "%s: cache codes must be 16-byte aligned", who);
+  return TVAE_OK;
+}
+bool rows_ok(const void* p, int64_t ldb, int64_t ldt, int64_t ldh, int dtype) {
+  const int64_t m = 16 / type_bytes(dtype);
+  return aligned16(p) && ldb % m == 0 && ldt % m == 0 && ldh % m == 0;
+}
+
+template <typename T, int DK>
+void launch_row(const AttnArgs& a, int kw, hipStream_t s) {
+  if (kw == 1)
+    hipLaunchKernelGGL((kv8_attn_row_kernel<T, DK, 1>), dim3((unsigned)((a.rows + 3) / 4), a.splits), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((kv8_attn_row_kernel<T, DK, 4>), dim3((unsigned)a.rows, a.splits), dim3(256), 0, s, a);
+}
+template <typename T>
+void launch_attn(const AttnArgs& a, int dk, hipStream_t s) {
+  const int kw = a.rows * a.splits >= 8192 ? 1 : 4;
+  if (dk == 32) launch_row<T, 32>(a, kw, s);
+  else if (dk == 64) launch_row<T, 64>(a, kw, s);
+  else if (dk == 128) launch_row<T, 128>(a, kw, s);
+  else launch_row<T, 256>(a, kw, s);
+  if (a.splits > 1) hipLaunchKernelGGL((kv8_attn_join_kernel<T>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a, dk);
+}
+
+}  // namespace
+
+extern "C" int tvae_kv8_store(const void* k, int64_t ldkb, int64_t ldkt, int64_t ldkh, const void* v, int64_t ldvb, int64_t ldvt,
+                              int64_t ldvh, int dtype, uint8_t* kc, uint8_t* vc, uint8_t* ke, uint8_t* ve, int n_pages,
+                              const int32_t* table, int per_seq, const int32_t* start, int start0, const int32_t* count, int n,
+                              int T, int h, int dk, int page, void* stream) {
+  TVAE_CHECK((k && v) || n == 0 || T == 0, TVAE_E_NULL, "tvae_kv8_store: null pointer");
+  const int rc = check_cache("tvae_kv8_store", kc, vc, ke, ve, n_pages, table, per_seq, n, h, dk, page, dtype);
+  if (rc) return rc;
+  TVAE_CHECK(T >= 0 && start0 >= 0 && (start || (int64_t)start0 + (count ? 0 : T) <= (int64_t)per_seq * page), TVAE_E_SHAPE,
+             "tvae_kv8_store: rows %d .. %lld do not fit %d pages of %d tokens", start0, (long long)start0 + T, per_seq, page);
+  TVAE_CHECK(rows_ok(k, ldkb, ldkt, ldkh, dtype) && rows_ok(v, ldvb, ldvt, ldvh, dtype), TVAE_E_SHAPE,
+             "tvae_kv8_store: k and v rows must be 16-byte aligned");
+  if (n == 0 || T == 0) return TVAE_OK;
+  const int slots = (T - 1 + page - 1) / page + 1;                      // pages that T rows can touch
+  const int64_t units = (int64_t)n * slots * h * 2;
+  TVAE_CHECK((units + 3) / 4 <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_store: too many pages in one call");
+  StoreArgs a = {{k, v}, {ldkb, ldvb}, {ldkt, ldvt}, {ldkh, ldvh}, {kc, vc}, {ke, ve}, {table, per_seq, n_pages}, start, count,
+                 start0, n, T, h, dk, page, slots};
+  const dim3 grid((unsigned)((units + 3) / 4));
+  if (dtype == TVAE_F32) hipLaunchKernelGGL(kv8_store_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else if (dtype == TVAE_BF16) hipLaunchKernelGGL(kv8_store_kernel<B16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(kv8_store_kernel<F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  TVAE_LAUNCH_CHECK("tvae_kv8_store");
+  return TVAE_OK;
+}
+
+extern "C" int tvae_kv8_load(const uint8_t* kc, const uint8_t* vc, const uint8_t* ke, const uint8_t* ve, int n_pages,
+                             const int32_t* table, int per_seq, const int32_t* start, int start0, const int32_t* count, void* k,
+                             void* v, int dtype, int n, int T, int h, int dk, int page, void* stream) {
+  TVAE_CHECK((k && v) || n == 0 || T == 0, TVAE_E_NULL, "tvae_kv8_load: null pointer");
+  const int rc = check_cache("tvae_kv8_load", kc, vc, ke, ve, n_pages, table, per_seq, n, h, dk, page, dtype);
+  if (rc) return rc;
+  TVAE_CHECK(T >= 0 && aligned16(k) && aligned16(v), TVAE_E_SHAPE, "tvae_kv8_load: T must not be negative, k and v 16-byte aligned");
+  if (n == 0 || T == 0) return TVAE_OK;
+  const int64_t blocks = ((int64_t)n * h * T * (dk / 4) + 255) / 256;
+  TVAE_CHECK(blocks <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_load: too many rows in one call");
+  LoadArgs a = {{kc, vc}, {ke, ve}, {k, v}, {table, per_seq, n_pages}, start, count, start0, n, T, h, dk, page};
+  const dim3 grid((unsigned)blocks, 2);
+  if (dtype == TVAE_F32) hipLaunchKernelGGL(kv8_load_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else if (dtype == TVAE_BF16) hipLaunchKernelGGL(kv8_load_kernel<B16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(kv8_load_kernel<F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  TVAE_LAUNCH_CHECK("tvae_kv8_load");
+  return TVAE_OK;
+}
+
+extern "C" int tvae_kv8_attn(const void* q, int64_t ldqb, int64_t ldqi, int64_t ldqh, void* o, int64_t ldob, int64_t ldoi,
+                             int64_t ldoh, int dtype, const uint8_t* kc, const uint8_t* vc, const uint8_t* ke, const uint8_t* ve,
+                             int n_pages, const int32_t* table, int per_seq, const int32_t* lens, int len0,
+                             const uint8_t* key_mask, int64_t ld_mask, int mask_w, int causal, int n, int h, int G, int Lq, int dk,
+                             int page, float scale, int splits, float* ws, void* stream) {
+  TVAE_CHECK((q && o) || n == 0 || Lq == 0, TVAE_E_NULL, "tvae_kv8_attn: null pointer");
+  const int rc = check_cache("tvae_kv8_attn", kc, vc, ke, ve, n_pages, table, per_seq, n, h, dk, page, dtype);
+  if (rc) return rc;
+  TVAE_CHECK(G >= 1 && Lq >= 0 && (int64_t)h * G <= INT32_MAX, TVAE_E_SHAPE, "tvae_kv8_attn: need G >= 1 and Lq >= 0 (G=%d Lq=%d)", G, Lq);
+  TVAE_CHECK(rows_ok(q, ldqb, ldqi, ldqh, dtype) && rows_ok(o, ldob, ldoi, ldoh, dtype), TVAE_E_SHAPE,
+             "tvae_kv8_attn: q and o rows must be 16-byte aligned");
+  TVAE_CHECK(lens || (len0 >= 0 && len0 <= (int64_t)per_seq * page), TVAE_E_SHAPE, "tvae_kv8_attn: %d keys do not fit %d pages of %d tokens",
+             len0, per_seq, page);
+  TVAE_CHECK(!key_mask || (mask_w >= 0 && ld_mask >= mask_w), TVAE_E_SHAPE, "tvae_kv8_attn: bad mask shape");
+  TVAE_CHECK(splits >= 1 && splits <= 1024 && (splits == 1 || ws), TVAE_E_SHAPE, "tvae_kv8_attn: 1 .. 1024 splits, more than one with a workspace");
+  const int64_t rows = (int64_t)n * Lq * h * G;
+  TVAE_CHECK((rows + 3) / 4 <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_attn: too many query rows in one call");
+  if (rows == 0) return TVAE_OK;
+  const int64_t cap = lens ? (int64_t)per_seq * page : len0;
+  int64_t chunk = ((cap + splits - 1) / splits + 127) / 128 * 128;
+  chunk = chunk < INT32_MAX ? chunk : INT32_MAX;
+  AttnArgs a = {q, o, ldqb, ldqi, ldqh, ldob, ldoi, ldoh, {kc, vc}, {ke, ve}, {table, per_seq, n_pages}, lens, key_mask, ws, rows,
+                ld_mask, mask_w, len0, causal, n, h, G, Lq, page, splits, (int)chunk, scale * 1.44269504088896341f};
+  if (dtype == TVAE_F32) launch_attn<float>(a, dk, (hipStream_t)stream);
+  else if (dtype == TVAE_BF16) launch_attn<B16>(a, dk, (hipStream_t)stream);
+  else launch_attn<F16>(a, dk, (hipStream_t)stream);
+  TVAE_LAUNCH_CHECK("tvae_kv8_attn");
+  return TVAE_OK;
+}

@@ -29,3 +29,30 @@ def vae_loss(x, x_out, mu, logvar, true_prop, pred_prop, weights, beta=1):
     total, bce, _, kld, mse = ops.LossFn.apply(x.long(), x_out, mu, logvar, None, true_prop, pred_prop,
                                                weights.to(torch.float32), float(beta), weights.shape[0] - 1, None)
     return total, bce, kld, mse
+
+
+MAX_TOP = 64
+
+
+def token_logprobs(logits, tokens=None, top=0):
+    """Log probabilities of given tokens under logits (..., V), with the entropy of every row and its `top` (0 .. 64) most likely
+    alternatives: ``(logp, entropy, top_logp, top_ids)`` of shapes (...), (...), (..., top), (..., top).
+
+    logits: float32, bfloat16 or float16; tokens: integer class ids (...), or None (logp is then 0).  A token outside [0, V) is
+    padding: its logp is 0 and passes no gradient, entropy and alternatives are the row's all the same.  Alternatives come in
+    descending order, equal logits in ascending order of their ids.  A class at -inf has probability 0 (and gradient 0); a
+    row of nothing else has logp -inf, entropy 0 and gradient 0; a NaN or +inf makes its row NaN.  Results are float32 (ids
+    int64).  logp, entropy and top_logp are differentiable in the logits, once.  No counterpart in the reference, whose
+    losses (transvae/loss.py:8-38) only give weighted means."""
+    if logits.dim() < 1 or logits.shape[-1] < 1 or logits.dtype not in ops.LOGIT_TYPES:
+        raise ops._lib.TvaeError("token_logprobs: logits must be float32, bfloat16 or float16 (..., V), got %s %s" % (tuple(logits.shape), logits.dtype))
+    V, lead = logits.shape[-1], logits.shape[:-1]
+    if not 0 <= top <= min(V, MAX_TOP):
+        raise ops._lib.TvaeError("token_logprobs: top must be in [0, min(V, %d)] (got %s for V = %d)" % (MAX_TOP, top, V))
+    if tokens is not None:
+        if tokens.shape != lead or tokens.is_floating_point() or tokens.dtype == torch.bool or tokens.device != logits.device:
+            raise ops._lib.TvaeError("token_logprobs: tokens must be integers of shape %s on %s, got %s %s on %s"
+                                     % (tuple(lead), logits.device, tuple(tokens.shape), tokens.dtype, tokens.device))
+        tokens = tokens.reshape(-1).long()
+    logp, entropy, top_logp, top_ids = ops.TokenLogpFn.apply(logits, tokens, int(top))
+    return logp.view(lead), entropy.view(lead), top_logp.view(*lead, top), top_ids.view(*lead, top)

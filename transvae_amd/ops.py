@@ -12,7 +12,7 @@ import os
 import torch
 
 from . import _lib
-from ._lib import (F32, BF16, F32X3, GEMM_B_SPLIT3, GEMM_B_BF16, GEMM_RELU, GEMM_ACCUM, GEMM_A_KMAJOR, GEMM_B_KMAJOR, GEMM_SPLITK,
+from ._lib import (F32, BF16, F32X3, F16, GEMM_B_SPLIT3, GEMM_B_BF16, GEMM_RELU, GEMM_ACCUM, GEMM_A_KMAJOR, GEMM_B_KMAJOR, GEMM_SPLITK,
                    GEMM_A_DROPMASK, GEMM_RELUMASK, call)
 
 # ----------------------------------------------------------------------------- configuration
@@ -152,6 +152,14 @@ def _stream():
     if _raw_stream is not None and _cur_device is not None:
         return C.c_void_p(_raw_stream(_cur_device()))
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def call_on(device, name, *args):
+    "one entry point on `device` and its current stream, whichever device is current (the stream is the last argument of all of them)"
+    if _cur_device is not None and _cur_device() == device.index:
+        return call(name, *args, _stream())
+    with torch.cuda.device(device):
+        call(name, *args, _stream())
 
 
 def _chk(t, name):
@@ -1283,6 +1291,67 @@ class LossFn(torch.autograd.Function):
         dpl = None if g["pred_len"] is None else g["pred_len"] * gt
         return (None, (g["logits"] * gt).view(ctx.shapes[0]), g["mu"] * gt, g["logvar"] * gt, dpl,
                 None, dpp, None, None, None, None)
+
+
+# ----------------------------------------------------------------------------- token log probabilities
+LOGIT_TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
+def _logit_rows(logits):
+    "(rows, V) view of the logits, dense in the class dimension (copied only if it is not), and its row stride"
+    V = logits.shape[-1]
+    lg = logits.reshape(-1, V)
+    if (V > 1 and lg.stride(1) != 1) or (lg.shape[0] > 1 and lg.stride(0) < V):
+        lg = lg.contiguous()
+    return lg, lg.stride(0) if lg.shape[0] > 1 else V
+
+
+def token_logp(logits, tokens, top=0, tok_sub=0, out=None):
+    """Raw launcher behind loss.token_logprobs: logits (rows, V) of row stride ld, tokens (rows,) int64 (any stride) or None, less
+    `tok_sub`.  Returns (logp, entropy, stat, top_logp, top_ids); `out` = (logp, entropy) may be strided (rows,) fp32 buffers."""
+    lg, ld = _logit_rows(logits)
+    rows, V = lg.shape
+    dev = lg.device
+    logp, entropy = out if out is not None else (torch.empty(rows, device=dev, dtype=torch.float32) for _ in range(2))
+    stat = torch.empty((rows, 2), device=dev, dtype=torch.float32)
+    top_logp = torch.empty((rows, top), device=dev, dtype=torch.float32)
+    top_ids = torch.empty((rows, top), device=dev, dtype=torch.int64)
+    segs = score_segments(rows, V)
+    ws = torch.empty(rows * segs * (3 + 2 * top), device=dev, dtype=torch.float32) if segs > 1 else None
+    call_on(dev, "tvae_token_logp", _p(lg), ld, LOGIT_TYPES[lg.dtype], _p(tokens), 1 if tokens is None else tokens.stride(0), int(tok_sub),
+            rows, V, top, _p(logp), logp.stride(0), _p(entropy), entropy.stride(0), _p(stat), _p(top_logp) if top else None,
+            _p(top_ids) if top else None, segs, _p(ws))
+    return logp, entropy, stat, top_logp, top_ids
+
+
+def score_segments(rows, V):
+    "parts that a row of V logits is cut into"
+    return max(1, min(-(-V // 8192), 1024 // max(1, rows)))
+
+
+class TokenLogpFn(torch.autograd.Function):
+    """token_logp with its gradient: dx_j = g_l (d_jy - p_j) - g_H p_j (ln p_j + H) + sum_t g_t (d_{j, i_t} - p_j)."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, top):
+        logp, entropy, stat, top_logp, top_ids = token_logp(logits, tokens, top)
+        ctx.save_for_backward(logits, tokens, stat, entropy, top_ids)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(top_ids)
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, tokens, stat, entropy, top_ids = ctx.saved_tensors
+        lg, ld = _logit_rows(logits)
+        rows, V = lg.shape
+        top = top_ids.shape[1]
+        dx = torch.empty((rows, V), device=lg.device, dtype=lg.dtype)
+        g_logp, g_entropy, g_top = (None if g is None else _c(g.to(torch.float32)) for g in (g_logp, g_entropy, g_top if top else None))
+        call_on(lg.device, "tvae_token_logp_bwd", _p(lg), ld, LOGIT_TYPES[lg.dtype], _p(tokens), 1 if tokens is None else tokens.stride(0), 0,
+                rows, V, top, _p(stat), _p(entropy), 1, _p(top_ids) if top else None, _p(g_logp), _p(g_entropy), _p(g_top), _p(dx))
+        return dx.view(logits.shape), None, None
 
 
 # ----------------------------------------------------------------------------- Adam
