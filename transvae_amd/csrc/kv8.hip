@@ -25,6 +25,7 @@ template <> struct Elem<float> {
     const float4 t = *reinterpret_cast<const float4*>(p);
     x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
   }
+  static __device__ inline void store4(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
   static __device__ inline void put(float* p, float x) { *p = x; }
 };
 template <> struct Elem<B16> {
@@ -39,6 +40,9 @@ template <> struct Elem<B16> {
     return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
   }
   static __device__ inline void put(B16* p, float x) { p->v = cvt(x); }
+  static __device__ inline void store4(B16* p, const float (&x)[4]) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(cvt(x[0]) | (uint32_t)cvt(x[1]) << 16, cvt(x[2]) | (uint32_t)cvt(x[3]) << 16);
+  }
 };
 template <> struct Elem<F16> {
   static __device__ inline void load4(const F16* p, float (&x)[4]) {
@@ -48,6 +52,10 @@ template <> struct Elem<F16> {
     for (int i = 0; i < 4; ++i) x[i] = (float)h[i];
   }
   static __device__ inline void put(F16* p, float x) { p->v = (_Float16)x; }
+  static __device__ inline void store4(F16* p, const float (&x)[4]) {
+    _Float16 h[4] = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+  }
 };
 
 __device__ inline float exp_scale(int e) { return __uint_as_float((uint32_t)e << 23); }          // 2^(e - 127)
@@ -395,6 +403,376 @@ __global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
   for (int c = 0; c < 16; ++c) Elem<T>::put(dst + c, o[c] * inv);
 }
 
+// ---- several query rows at once, on the matrix cores
+typedef __bf16 bfx2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bfx8 __attribute__((ext_vector_type(8)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+
+union Frag {                 // eight bf16 of one lane: an operand of v_mfma_f32_16x16x32_bf16
+  uint32_t u[4];
+  bfx2 h[4];
+  bfx8 v;
+};
+// how many bf16 pieces a query, and a weight, is cut into.  A code is exact in bf16, so only the other operand decides the
+// products' precision: fp32 = three pieces of 8 bits (exact), fp16 queries = two (exact) and weights to 2^-16, bf16 = itself.
+template <typename T> struct Pieces;
+template <> struct Pieces<float> { static constexpr int Q = 3, P = 3; };
+template <> struct Pieces<F16> { static constexpr int Q = 2, P = 2; };
+template <> struct Pieces<B16> { static constexpr int Q = 1, P = 1; };
+
+// piece k of 8 values; with more than one piece each takes the next 8 bits (cut off, so the rest is exact), a single one rounds
+template <int N>
+__device__ inline void cut_pieces(const float (&x)[8], Frag (&f)[N]) {
+  if (N == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const floatx2 t = {x[2 * i], x[2 * i + 1]};
+      f[0].h[i] = __builtin_convertvector(t, bfx2);
+    }
+    return;
+  }
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[k].u[i] = __builtin_amdgcn_perm(__float_as_uint(r[2 * i + 1]), __float_as_uint(r[2 * i]), 0x07060302u);
+      if (k + 1 < N) {
+        r[2 * i] -= __uint_as_float(__float_as_uint(r[2 * i]) & 0xFFFF0000u);
+        r[2 * i + 1] -= __uint_as_float(__float_as_uint(r[2 * i + 1]) & 0xFFFF0000u);
+      }
+    }
+  }
+}
+__device__ inline float quad_max(float x) {        // over the four lanes of a column (lane & 15)
+  uintx2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float quad_sum(float x) {
+  uintx2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The codes of 32 tokens as one lane (c = lane & 15, quad = lane >> 4) loads them: for the scores the token rows 8 (c >> 2) +
+// 4 t + (c & 3), t = 0, 1, 16 codes of every 64; for the second product W = DK / 16 codes of each of the tokens 8 quad .. + 7.
+template <int DK>
+struct CodeTile {
+  static constexpr int KW4 = DK / 16, VW = DK / 16 >= 4 ? DK / 64 : 1;   // dwords of a token row, and of W codes
+  uint32_t k[2][KW4 >= 4 ? KW4 : 2];
+  uint32_t v[8][VW];
+  float ks, vs;              // scales of the lane's tokens 8 quad .. + 7
+  bool have;                 // their page exists
+};
+
+template <int DK>
+__device__ inline void load_tile(CodeTile<DK>& t, const AttnArgs& a, int head, int idk, int idv, int64_t t0, int c, int quad) {
+  constexpr int W = DK / 16;
+  const int pm = a.page - 1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int w = 0; w < (W >= 4 ? W : 2); ++w) t.k[i][w] = 0;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+#pragma unroll
+    for (int w = 0; w < CodeTile<DK>::VW; ++w) t.v[j][w] = 0;
+  }
+  t.ks = t.vs = 0.f;
+  t.have = idv >= 0;
+  if (idk >= 0) {
+    const uint8_t* p = a.codes[0] + (((size_t)idk * a.h + head) * a.page + ((int)(t0 + 8 * (c >> 2)) & pm) + (c & 3)) * DK;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* r = p + 4 * i * DK;
+      if (DK == 32) {
+        *reinterpret_cast<uint2*>(t.k[i]) = *reinterpret_cast<const uint2*>(r + 8 * quad);
+      } else {
+#pragma unroll
+        for (int w = 0; w < DK / 64; ++w) *reinterpret_cast<uint4*>(t.k[i] + 4 * w) = *reinterpret_cast<const uint4*>(r + 64 * w + 16 * quad);
+      }
+    }
+  }
+  if (idv >= 0) {
+    const size_t ph = (size_t)idv * a.h + head;
+    const uint8_t* p = a.codes[1] + (ph * a.page + ((int)(t0 + 8 * quad) & pm)) * DK + W * c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (W == 2) t.v[j][0] = *reinterpret_cast<const uint16_t*>(p + j * DK);
+      else if (W == 4) t.v[j][0] = *reinterpret_cast<const uint32_t*>(p + j * DK);
+      else if (W == 8) *reinterpret_cast<uint2*>(t.v[j]) = *reinterpret_cast<const uint2*>(p + j * DK);
+      else *reinterpret_cast<uint4*>(t.v[j]) = *reinterpret_cast<const uint4*>(p + j * DK);
+    }
+    t.ks = exp_scale(a.exps[0][ph]);
+    t.vs = exp_scale(a.exps[1][ph]);
+  }
+}
+
+// G * Lq query rows of one (sequence, key head) share its codes: NT tiles of 16 rows a wave.  Both products are taken
+// transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane's scores (4 + 4 tokens of one query) are in place as the second
+// product's operand and no weight crosses lanes; codes go from memory to registers to the matrix cores (a byte permute turns
+// the eight token rows of V into columns), nothing is staged in shared memory.  The running maximum is only raised when a
+// score passes it by 2^8: until then weights just exceed 1, which costs no precision and saves the rescaling.
+// KW = 4: the block's waves take every fourth group of 32 tokens and meet at the end; KW = 1: every wave has rows of its own.
+template <typename T, int DK, int NT, int KW>
+__global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
+  constexpr int W = DK / 16, KS = DK / 32, NQ = Pieces<T>::Q, NP = Pieces<T>::P, VW = CodeTile<DK>::VW;
+  constexpr int REGS = NT * (4 * W + 2);
+  __shared__ float buf[KW == 1 ? 1 : 2 * REGS * 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, quad = lane >> 4;
+  const int M = a.G * a.Lq, mt = (M + 16 * NT - 1) / (16 * NT);
+  int64_t unit = KW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (unit >= (int64_t)a.n * a.h * mt) return;                          // KW == 4: one unit a block, uniform
+  const int kw = KW == 1 ? 0 : wave, split = blockIdx.y;
+  const int64_t bh_m = unit;
+  const int r0 = (int)(bh_m % mt) * 16 * NT;
+  unit /= mt;
+  const int head = (int)(unit % a.h), b = (int)(unit / a.h);
+  const int len = seq_len(a, b);
+  const int64_t beg = (int64_t)split * a.chunk;
+  auto end_of = [&](int r) {                                            // tokens that row r sees, in this part
+    const int64_t e = len - (a.causal ? a.Lq - 1 - r / a.G : 0);
+    return (int)(e < beg + a.chunk ? e : beg + a.chunk);
+  };
+  const int rl = r0 + 16 * NT - 1 < M ? r0 + 16 * NT - 1 : M - 1;
+  const int most = end_of(rl), least = end_of(r0);
+  Frag qf[NT][KS][NQ];
+  int end[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + 16 * t + c;
+    end[t] = r < M ? end_of(r) : 0;
+    const int rr = r < M ? r : M - 1;
+    const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)b * a.ldqb + (int64_t)(rr / a.G) * a.ldqi + (int64_t)(head * a.G + rr % a.G) * a.ldqh;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = DK == 32 ? 8 * quad : 64 * (s >> 1) + 16 * quad + 8 * (s & 1);
+      float x[8], y[4];
+      Elem<T>::load4(q + d, y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = y[i];
+      Elem<T>::load4(q + d + 4, y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 + i] = y[i];
+      cut_pieces<NQ>(x, qf[t][s]);
+    }
+  }
+  floatx4 o[NT][W];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int g = 0; g < W; ++g) o[t][g] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int shift = 31 - __clz(a.page);
+  auto page_at = [&](int64_t tok) { return tok < most ? a.pages.at(b, (int)(tok >> shift)) : -1; };
+  const int64_t step = 32 * KW;
+  int64_t t0 = beg + 32 * kw;
+  CodeTile<DK> cur, nxt;
+  load_tile<DK>(cur, a, head, page_at(t0 + 8 * (c >> 2)), page_at(t0 + 8 * quad), t0, c, quad);
+  int idk = page_at(t0 + step + 8 * (c >> 2)), idv = page_at(t0 + step + 8 * quad);
+  for (; t0 < most; t0 += step) {
+    load_tile<DK>(nxt, a, head, idk, idv, t0 + step, c, quad);
+    idk = page_at(t0 + 2 * step + 8 * (c >> 2));
+    idv = page_at(t0 + 2 * step + 8 * quad);
+    // scores: sc[t][i] is the lane's query c of tile t against token t0 + 8 quad + i
+    floatx4 sc[NT][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sc[t][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        Frag kf;
+        kf.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s], 1.f, false);
+        kf.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s], 1.f, true);
+        kf.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s + 1], 1.f, false);
+        kf.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s + 1], 1.f, true);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int p = NQ - 1; p >= 0; --p)
+            sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.v, qf[t][s][p].v, sc[t][i], 0, 0, 0);
+        }
+      }
+    }
+    const bool plain = t0 + 32 <= least && !a.mask && __all(cur.have);  // every row of the unit sees all 32 tokens
+    uint32_t seen = 0xFF;                                               // bit i: token 8 quad + i exists and is not masked
+    if (!plain) {
+      if (!cur.have) seen = 0;
+      if (a.mask) {
+        const uint8_t* mk = a.mask + (int64_t)b * a.ld_mask;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int64_t j = t0 + 8 * quad + i;
+          if (!(j < most && j < a.mask_w && mk[j] != 0)) seen &= ~(1u << i);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {                                     // codes that no row sees: 0 * NaN would not vanish
+        if (!(t0 + 8 * quad + i < most) || !(seen >> i & 1)) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) cur.v[i][w] = 0;
+        }
+      }
+    }
+    const float ksc = cur.ks * a.scale;
+    Frag pf[NT][NP];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3] * ksc;
+      if (!plain) {
+        const int64_t left = end[t] - (t0 + 8 * quad);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (i < left && (seen >> i & 1)) ? x[i] : -INFINITY;
+      }
+      float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      if (__any(mx > m[t] + 8.f)) {
+        mx = fmaxf(m[t], quad_max(mx));
+        const float al = __builtin_amdgcn_exp2f(m[t] - (mx == -INFINITY ? 0.f : mx));
+        m[t] = mx;
+        l[t] *= al;
+#pragma unroll
+        for (int g = 0; g < W; ++g) o[t][g] *= al;
+      }
+      const float ms = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(x[i] - ms);
+        l[t] += x[i];
+      }
+      cut_pieces<NP>(x, pf[t]);
+    }
+    // a token that some rows see and others do not, whose value is NaN: take it out here and put it back below
+    bool strange = false;
+    if (!plain && least < most && t0 + 32 > least) {
+      uint32_t hit = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) hit |= ((cur.v[i][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+      }
+      strange = __any(hit != 0);
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      uint32_t lo[4], hi[4];                                            // bytes {x0, y0, x1, y1} and {x2, y2, x3, y3} of two tokens' dwords
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = __builtin_amdgcn_perm(cur.v[2 * i + 1][w], cur.v[2 * i][w], 0x05010400u);
+        hi[i] = __builtin_amdgcn_perm(cur.v[2 * i + 1][w], cur.v[2 * i][w], 0x07030602u);
+      }
+#pragma unroll
+      for (int g = 0; g < (W < 4 ? W : 4); ++g) {
+        Frag vf;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t src = g < 2 ? lo[i] : hi[i];
+          vf.h[i] = g & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, cur.vs, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, cur.vs, false);
+        }
+        Frag nan;
+        if (strange) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {                                 // 1 where the value is NaN, and the value 0 there
+            const bool n0 = (vf.u[i] & 0x7FFFu) > 0x7F80u, n1 = (vf.u[i] >> 16 & 0x7FFFu) > 0x7F80u;
+            nan.u[i] = (n0 ? 0x3F80u : 0u) | (n1 ? 0x3F800000u : 0u);
+            vf.u[i] &= (n0 ? 0u : 0xFFFFu) | (n1 ? 0u : 0xFFFF0000u);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p)
+            o[t][4 * w + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[t][p].v, o[t][4 * w + g], 0, 0, 0);
+          if (strange) {
+            Frag see;
+            const int64_t left = end[t] - (t0 + 8 * quad);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              see.u[i] = (2 * i < left && (seen >> (2 * i) & 1) ? 0x3F80u : 0u) | (2 * i + 1 < left && (seen >> (2 * i + 1) & 1) ? 0x3F800000u : 0u);
+            floatx4 cnt = floatx4{0.f, 0.f, 0.f, 0.f};
+            cnt = __builtin_amdgcn_mfma_f32_16x16x32_bf16(nan.v, see.v, cnt, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (cnt[e] > 0.f) o[t][4 * w + g][e] = __uint_as_float(0x7FC00000u);
+          }
+        }
+      }
+    }
+    cur = nxt;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) l[t] = quad_sum(l[t]);
+  if (KW > 1) {                                                         // waves 2, 3 hand over to 0, 1, then 1 to 0
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+      float* dst = buf + (wave & (half - 1)) * REGS * 64 + lane;
+      if (wave >= half && wave < 2 * half) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int g = 0; g < W; ++g) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[(t * (4 * W + 2) + 4 * g + e) * 64] = o[t][g][e];
+          }
+          dst[(t * (4 * W + 2) + 4 * W) * 64] = m[t];
+          dst[(t * (4 * W + 2) + 4 * W + 1) * 64] = l[t];
+        }
+      }
+      __syncthreads();
+      if (wave < half) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float m2 = dst[(t * (4 * W + 2) + 4 * W) * 64], l2 = dst[(t * (4 * W + 2) + 4 * W + 1) * 64];
+          const float mm = fmaxf(m[t], m2), z = mm == -INFINITY ? 0.f : mm;
+          const float f1 = __builtin_amdgcn_exp2f(m[t] - z), f2 = __builtin_amdgcn_exp2f(m2 - z);
+          m[t] = mm;
+          l[t] = l[t] * f1 + l2 * f2;
+#pragma unroll
+          for (int g = 0; g < W; ++g) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][g][e] = o[t][g][e] * f1 + dst[(t * (4 * W + 2) + 4 * g + e) * 64] * f2;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (wave != 0) return;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + 16 * t + c;
+    if (r >= M) continue;
+    const int64_t row = ((int64_t)b * a.h + head) * M + r;
+    float* part = a.splits > 1 ? a.ws + (row * a.splits + split) * DK + 4 * W * quad : nullptr;
+    T* dst = reinterpret_cast<T*>(a.o) + (int64_t)b * a.ldob + (int64_t)(r / a.G) * a.ldoi + (int64_t)(head * a.G + r % a.G) * a.ldoh + 4 * W * quad;
+    const float inv = part ? 1.f : l[t] == 0.f ? 0.f : 1.f / l[t];
+#pragma unroll
+    for (int i = 0; i < 4 * W; i += 4) {                                // dimension W e + g of the lane's 4 W
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = o[t][(i + e) % W][(i + e) / W] * inv;
+      if (part) *reinterpret_cast<float4*>(part + i) = make_float4(y[0], y[1], y[2], y[3]);
+      else Elem<T>::store4(dst + i, y);
+    }
+    if (part && quad == 0) {
+      float* ml = a.ws + a.rows * a.splits * DK + (row * a.splits + split) * 2;
+      ml[0] = m[t];
+      ml[1] = l[t];
+    }
+  }
+}
+
 // joins the parts of a split row: one wave a row
 template <typename T>
 __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a, int dk) {
@@ -447,19 +825,36 @@ bool rows_ok(const void* p, int64_t ldb, int64_t ldt, int64_t ldh, int dtype) {
 }
 
 template <typename T, int DK>
-void launch_row(const AttnArgs& a, int kw, hipStream_t s) {
-  if (kw == 1)
+void launch_row(const AttnArgs& a, hipStream_t s) {
+  if (a.rows * a.splits >= 8192)
     hipLaunchKernelGGL((kv8_attn_row_kernel<T, DK, 1>), dim3((unsigned)((a.rows + 3) / 4), a.splits), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((kv8_attn_row_kernel<T, DK, 4>), dim3((unsigned)a.rows, a.splits), dim3(256), 0, s, a);
 }
+template <typename T, int DK, int NT>
+void launch_tile(const AttnArgs& a, hipStream_t s) {
+  const int64_t units = (int64_t)a.n * a.h * ((a.G * a.Lq + 16 * NT - 1) / (16 * NT));
+  if (units * a.splits >= 8192)
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 1>), dim3((unsigned)((units + 3) / 4), a.splits), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 4>), dim3((unsigned)units, a.splits), dim3(256), 0, s, a);
+}
+template <typename T, int DK>
+void launch_dk(const AttnArgs& a, hipStream_t s) {
+  // tiles of 16 rows a wave: as many as its registers take (queries, sums, scores: DK / 32 * pieces * 4 + DK / 4 + 8 a tile)
+  constexpr int PER = DK / 32 * Pieces<T>::Q * 4 + DK / 4 + 8, MOST = 4 * PER <= 150 ? 4 : 2 * PER <= 150 ? 2 : 1;
+  const int M = a.G * a.Lq;
+  if (M == 1) launch_row<T, DK>(a, s);
+  else if (M <= 16 || MOST == 1) launch_tile<T, DK, 1>(a, s);
+  else if (M <= 32 || MOST == 2) launch_tile<T, DK, MOST == 1 ? 1 : 2>(a, s);
+  else launch_tile<T, DK, MOST>(a, s);
+}
 template <typename T>
 void launch_attn(const AttnArgs& a, int dk, hipStream_t s) {
-  const int kw = a.rows * a.splits >= 8192 ? 1 : 4;
-  if (dk == 32) launch_row<T, 32>(a, kw, s);
-  else if (dk == 64) launch_row<T, 64>(a, kw, s);
-  else if (dk == 128) launch_row<T, 128>(a, kw, s);
-  else launch_row<T, 256>(a, kw, s);
+  if (dk == 32) launch_dk<T, 32>(a, s);
+  else if (dk == 64) launch_dk<T, 64>(a, s);
+  else if (dk == 128) launch_dk<T, 128>(a, s);
+  else launch_dk<T, 256>(a, s);
   if (a.splits > 1) hipLaunchKernelGGL((kv8_attn_join_kernel<T>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a, dk);
 }
 
