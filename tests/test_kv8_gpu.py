@@ -231,6 +231,43 @@ def test_what_is_dead_or_masked_never_matters(Lq, G):
     assert bool(((o.cpu().double() - clean[0]).abs() <= attend_bound(*clean, dk, per * page, torch.float32)).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Lq,G,dk", [(1, 1, 64), (1, 8, 128), (6, 3, 64), (40, 1, 32), (3, 1, 256)])
+def test_a_nan_key_or_value_reaches_the_queries_that_see_it(Lq, G, dk, dtype):
+    "causal queries in front of it, masked tokens, pages of masked tokens only (whatever their exponents)"
+    n, h, page, per = 2, 2, 16, 6
+    gpu, ref, _, _ = pair(n, per, h, dk, page, False)
+    fill(gpu, ref)
+    L = per * page - 3
+    mask = torch.ones((n, L), dtype=torch.bool)
+    mask[1, 2 * page:3 * page] = False
+    mask[0, 5] = False
+    gpu.k[per + 2], gpu.v[per + 2], gpu.k_exp[per + 2], gpu.v_exp[per + 2] = 127, 255, 255, 255
+    gpu.v[0, :, 5], gpu.k[0, :, 5] = 127, 127
+    q = (torch.randn((n, Lq, h * G, dk), generator=torch.Generator().manual_seed(1)) * 0.2).to(dtype)
+    lim = None
+    for at in (L - 1, L - 2, L - min(Lq, 20)):                     # seen by the last 1, 2, min(Lq, 20) queries
+        page_at, row = divmod(at, page)
+        saved = gpu.v[page_at, 1, row, 3].clone()
+        gpu.v[page_at, 1, row, 3] = 127
+        o = gpu.attend(q.cuda(), L, key_mask=mask.cuda()).cpu()
+        gpu.v[page_at, 1, row, 3] = saved
+        want, wv, qk = ref.attend(q, [L] * n, None, per, True, mask)
+        hit = torch.zeros_like(want, dtype=torch.bool)
+        hit[0, at - (L - Lq) if at >= L - Lq else 0:, G:, 3] = True
+        assert torch.equal(torch.isnan(o), hit), (at, torch.isnan(o).nonzero()[:5], hit.nonzero()[:5])
+        lim = attend_bound(want, wv, qk, dk, L, dtype)
+        assert bool((((o.double() - want).abs() <= lim) | hit).all())
+        saved = gpu.k[page_at, 0, row, 3].clone()
+        gpu.k[page_at, 0, row, 3] = 255
+        o = gpu.attend(q.cuda(), L, key_mask=mask.cuda()).cpu()
+        gpu.k[page_at, 0, row, 3] = saved
+        hit[:] = False
+        hit[0, at - (L - Lq) if at >= L - Lq else 0:, :G] = True
+        assert torch.equal(torch.isnan(o), hit)
+        assert bool((((o.double() - want).abs() <= lim) | hit).all())
+
+
 def test_values_of_a_visible_nan_reach_their_own_row_only():
     n, h, dk, page = 2, 2, 64, 32
     gpu, ref, _, _ = pair(n, 2, h, dk, page, False)

@@ -96,6 +96,21 @@ struct Pages {
     return p >= 0 && p < n_pages ? p : -1;                   // -1: no such page, nothing is read or written
   }
 };
+// The same in two halves and without a branch, so that a lookup is in flight while something else is computed: ask() loads a
+// table entry (any one where there is no table: `spare` is readable memory), page() makes the id of it.
+struct PageRow {
+  const int32_t* row;
+  int base, last, n_pages;
+  bool tabled;
+  __device__ inline PageRow(const Pages& p, int b, const void* spare)
+      : row(p.table ? p.table + (size_t)b * p.per_seq : reinterpret_cast<const int32_t*>(spare)), base(b * p.per_seq), last(p.per_seq - 1),
+        n_pages(p.n_pages), tabled(p.table != nullptr) {}
+  __device__ inline int ask(int slot) const { return row[tabled ? (slot < last ? slot : last) : 0]; }
+  __device__ inline int page(int raw, int slot, bool want) const {
+    const int p = tabled ? raw : base + slot;
+    return want && p >= 0 && p < n_pages ? p : -1;
+  }
+};
 
 // ------------------------------------------------------------------------------------------------ store
 struct StoreArgs {
@@ -288,29 +303,36 @@ __global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
   float m = -INFINITY, l = 0.f, o[16];
 #pragma unroll
   for (int d = 0; d < 16; ++d) o[d] = 0.f;
+  const PageRow pages(a.pages, b, a.codes[0]);
+  const int shift = 31 - __clz(a.page), pm = a.page - 1;
+  const uint8_t* mk = a.mask ? a.mask + (int64_t)b * a.ld_mask : a.exps[0];
   for (int64_t j0 = beg + (int64_t)kw * KPI; j0 < end; j0 += (int64_t)KW * KPI) {
+    // every load goes out without a branch; a key that is not visible reads page 0 instead, which all such keys share
     uint4 kc[U], vc[U];
-    float ks[U], vs[U], s[U];
+    int raw[U], ek[U], ev[U], slot[U];
+    uint8_t mb[U];
+    float s[U];
     bool vis[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t j = j0 + u * NK + kg;
-      bool see = j < end;
-      if (see && a.mask) see = j < a.mask_w && a.mask[(int64_t)b * a.ld_mask + j] != 0;
-      int id = -1;
-      if (see) id = a.pages.at(b, (int)(j / a.page));
-      see = id >= 0;
-      kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
-      ks[u] = vs[u] = 0.f;
-      if (see) {
-        const size_t ph = (size_t)id * a.h + head;
-        const size_t off = (ph * a.page + (int)(j % a.page)) * DK + 16 * part;
-        kc[u] = *reinterpret_cast<const uint4*>(a.codes[0] + off);
-        vc[u] = *reinterpret_cast<const uint4*>(a.codes[1] + off);
-        ks[u] = exp_scale(a.exps[0][ph]);
-        vs[u] = exp_scale(a.exps[1][ph]);
-      }
-      vis[u] = see;
+      vis[u] = j < end;
+      const int jj = vis[u] ? (int)j : 0;
+      slot[u] = jj >> shift;
+      raw[u] = pages.ask(slot[u]);
+      mb[u] = mk[a.mask ? (jj < a.mask_w ? jj : 0) : 0];
+      if (a.mask) vis[u] = vis[u] && jj < a.mask_w;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int id = pages.page(raw[u], slot[u], vis[u] && (!a.mask || mb[u] != 0));
+      vis[u] = id >= 0;
+      const size_t ph = vis[u] ? (size_t)id * a.h + head : 0;
+      const size_t off = vis[u] ? (ph * a.page + ((int)(j0 + u * NK + kg) & pm)) * DK + 16 * part : 16 * part;
+      kc[u] = *reinterpret_cast<const uint4*>(a.codes[0] + off);
+      vc[u] = *reinterpret_cast<const uint4*>(a.codes[1] + off);
+      ek[u] = a.exps[0][ph];
+      ev[u] = a.exps[1][ph];
     }
     float mn = m;
 #pragma unroll
@@ -324,7 +346,7 @@ __global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc = fmaf(x[e], qr[4 * c + e], acc);
       }
-      acc = group_sum<LPK>(acc) * (ks[u] * a.scale);
+      acc = group_sum<LPK>(acc) * (exp_scale(ek[u]) * a.scale);
       s[u] = vis[u] ? acc : -INFINITY;
       mn = fmaxf(mn, s[u]);
     }
@@ -338,8 +360,8 @@ __global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
     for (int u = 0; u < U; ++u) {
       const float p = __builtin_amdgcn_exp2f(s[u] - ms);
       l += p;
-      const float pv = p * vs[u];
-      const uint32_t w[4] = {vc[u].x, vc[u].y, vc[u].z, vc[u].w};
+      const float pv = vis[u] ? p * exp_scale(ev[u]) : 0.f;
+      const uint32_t w[4] = {vis[u] ? vc[u].x : 0u, vis[u] ? vc[u].y : 0u, vis[u] ? vc[u].z : 0u, vis[u] ? vc[u].w : 0u};   // 0 * NaN would not vanish
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         float x[4];
@@ -463,54 +485,48 @@ __device__ inline float quad_sum(float x) {
 // 4 t + (c & 3), t = 0, 1, 16 codes of every 64; for the second product W = DK / 16 codes of each of the tokens 8 quad .. + 7.
 template <int DK>
 struct CodeTile {
-  static constexpr int KW4 = DK / 16, VW = DK / 16 >= 4 ? DK / 64 : 1;   // dwords of a token row, and of W codes
-  uint32_t k[2][KW4 >= 4 ? KW4 : 2];
+  static constexpr int W = DK / 16, KN = W >= 4 ? W : 2, VW = W >= 4 ? DK / 64 : 1;     // dwords of a lane's token row, and of W codes
+  uint32_t k[2][KN];
   uint32_t v[8][VW];
-  float ks, vs;              // scales of the lane's tokens 8 quad .. + 7
+  int ek, ev;                // exponents of the lane's tokens 8 quad .. + 7
   bool have;                 // their page exists
-};
 
-template <int DK>
-__device__ inline void load_tile(CodeTile<DK>& t, const AttnArgs& a, int head, int idk, int idv, int64_t t0, int c, int quad) {
-  constexpr int W = DK / 16;
-  const int pm = a.page - 1;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int w = 0; w < (W >= 4 ? W : 2); ++w) t.k[i][w] = 0;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-#pragma unroll
-    for (int w = 0; w < CodeTile<DK>::VW; ++w) t.v[j][w] = 0;
-  }
-  t.ks = t.vs = 0.f;
-  t.have = idv >= 0;
-  if (idk >= 0) {
-    const uint8_t* p = a.codes[0] + (((size_t)idk * a.h + head) * a.page + ((int)(t0 + 8 * (c >> 2)) & pm) + (c & 3)) * DK;
+  // idk, idv: pages of the tokens that the lane loads for the scores and for the second product; -1 reads page 0 instead
+  __device__ inline void load(const AttnArgs& a, int head, int idk, int idv, int64_t t0, int c, int quad) {
+    const int pm = a.page - 1;
+    have = idv >= 0;
+    const size_t pk = ((size_t)(idk < 0 ? 0 : idk) * a.h + head) * a.page, ph = (size_t)(idv < 0 ? 0 : idv) * a.h + head;
+    const uint8_t* p = a.codes[0] + (pk + ((int)(t0 + 8 * (c >> 2)) & pm) + (c & 3)) * DK;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint8_t* r = p + 4 * i * DK;
       if (DK == 32) {
-        *reinterpret_cast<uint2*>(t.k[i]) = *reinterpret_cast<const uint2*>(r + 8 * quad);
+        *reinterpret_cast<uint2*>(k[i]) = *reinterpret_cast<const uint2*>(r + 8 * quad);
       } else {
 #pragma unroll
-        for (int w = 0; w < DK / 64; ++w) *reinterpret_cast<uint4*>(t.k[i] + 4 * w) = *reinterpret_cast<const uint4*>(r + 64 * w + 16 * quad);
+        for (int w = 0; w < DK / 64; ++w) *reinterpret_cast<uint4*>(k[i] + 4 * w) = *reinterpret_cast<const uint4*>(r + 64 * w + 16 * quad);
       }
     }
-  }
-  if (idv >= 0) {
-    const size_t ph = (size_t)idv * a.h + head;
-    const uint8_t* p = a.codes[1] + (ph * a.page + ((int)(t0 + 8 * quad) & pm)) * DK + W * c;
+    ek = a.exps[0][ph];
+    p = a.codes[1] + (ph * a.page + ((int)(t0 + 8 * quad) & pm)) * DK + W * c;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (W == 2) t.v[j][0] = *reinterpret_cast<const uint16_t*>(p + j * DK);
-      else if (W == 4) t.v[j][0] = *reinterpret_cast<const uint32_t*>(p + j * DK);
-      else if (W == 8) *reinterpret_cast<uint2*>(t.v[j]) = *reinterpret_cast<const uint2*>(p + j * DK);
-      else *reinterpret_cast<uint4*>(t.v[j]) = *reinterpret_cast<const uint4*>(p + j * DK);
+      if (W == 2) v[j][0] = *reinterpret_cast<const uint16_t*>(p + j * DK);
+      else if (W == 4) v[j][0] = *reinterpret_cast<const uint32_t*>(p + j * DK);
+      else if (W == 8) *reinterpret_cast<uint2*>(v[j]) = *reinterpret_cast<const uint2*>(p + j * DK);
+      else *reinterpret_cast<uint4*>(v[j]) = *reinterpret_cast<const uint4*>(p + j * DK);
     }
-    t.ks = exp_scale(a.exps[0][ph]);
-    t.vs = exp_scale(a.exps[1][ph]);
+    ev = a.exps[1][ph];
+  }
+};
+
+// Eight tokens' W codes as operands of the second product: group g is dimension W c + g of tokens 8 quad .. + 7, in bf16, scaled.
+template <int DK>
+__device__ inline void value_frag(Frag& f, const uint32_t (&v)[8][CodeTile<DK>::VW], int w, int g, float scale) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {                                         // bytes {x0, y0, x1, y1} or {x2, y2, x3, y3} of two tokens
+    const uint32_t two = __builtin_amdgcn_perm(v[2 * i + 1][w], v[2 * i][w], g < 2 ? 0x05010400u : 0x07030602u);
+    f.h[i] = g & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, scale, false);
   }
 }
 
@@ -522,7 +538,7 @@ __device__ inline void load_tile(CodeTile<DK>& t, const AttnArgs& a, int head, i
 // KW = 4: the block's waves take every fourth group of 32 tokens and meet at the end; KW = 1: every wave has rows of its own.
 template <typename T, int DK, int NT, int KW>
 __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
-  constexpr int W = DK / 16, KS = DK / 32, NQ = Pieces<T>::Q, NP = Pieces<T>::P, VW = CodeTile<DK>::VW;
+  constexpr int W = DK / 16, KS = DK / 32, NQ = Pieces<T>::Q, NP = Pieces<T>::P, VW = CodeTile<DK>::VW, VG = W < 4 ? W : 4;
   constexpr int REGS = NT * (4 * W + 2);
   __shared__ float buf[KW == 1 ? 1 : 2 * REGS * 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, quad = lane >> 4;
@@ -573,16 +589,21 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
     for (int g = 0; g < W; ++g) o[t][g] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
   const int shift = 31 - __clz(a.page);
-  auto page_at = [&](int64_t tok) { return tok < most ? a.pages.at(b, (int)(tok >> shift)) : -1; };
+  const PageRow pages(a.pages, b, a.codes[0]);
   const int64_t step = 32 * KW;
   int64_t t0 = beg + 32 * kw;
+  const int ofk = 8 * (c >> 2), ofv = 8 * quad;
+  auto ask = [&](int64_t tok) { return pages.ask(tok < most ? (int)(tok >> shift) : 0); };
+  auto page = [&](int raw, int64_t tok) { return pages.page(raw, (int)(tok >> shift), tok < most); };
+  // page ids are looked up two groups ahead, codes loaded one group ahead
   CodeTile<DK> cur, nxt;
-  load_tile<DK>(cur, a, head, page_at(t0 + 8 * (c >> 2)), page_at(t0 + 8 * quad), t0, c, quad);
-  int idk = page_at(t0 + step + 8 * (c >> 2)), idv = page_at(t0 + step + 8 * quad);
+  int rk = ask(t0 + ofk), rv = ask(t0 + ofv);
+  cur.load(a, head, page(rk, t0 + ofk), page(rv, t0 + ofv), t0, c, quad);
+  rk = ask(t0 + step + ofk), rv = ask(t0 + step + ofv);
   for (; t0 < most; t0 += step) {
-    load_tile<DK>(nxt, a, head, idk, idv, t0 + step, c, quad);
-    idk = page_at(t0 + 2 * step + 8 * (c >> 2));
-    idv = page_at(t0 + 2 * step + 8 * quad);
+    const int idk = page(rk, t0 + step + ofk), idv = page(rv, t0 + step + ofv);
+    rk = ask(t0 + 2 * step + ofk), rv = ask(t0 + 2 * step + ofv);
+    nxt.load(a, head, idk, idv, t0 + step, c, quad);
     // scores: sc[t][i] is the lane's query c of tile t against token t0 + 8 quad + i
     floatx4 sc[NT][2];
 #pragma unroll
@@ -610,11 +631,15 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
       if (!cur.have) seen = 0;
       if (a.mask) {
         const uint8_t* mk = a.mask + (int64_t)b * a.ld_mask;
+        uint8_t mb[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int64_t j = t0 + 8 * quad + i;
-          if (!(j < most && j < a.mask_w && mk[j] != 0)) seen &= ~(1u << i);
+          mb[i] = mk[j < a.mask_w ? j : 0];
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (t0 + 8 * quad + i >= a.mask_w || mb[i] == 0) seen &= ~(1u << i);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {                                     // codes that no row sees: 0 * NaN would not vanish
@@ -624,7 +649,7 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
         }
       }
     }
-    const float ksc = cur.ks * a.scale;
+    const float ksc = exp_scale(cur.ek) * a.scale, vsc = seen ? exp_scale(cur.ev) : 1.f;   // a page of masked tokens may hold any exponent
     Frag pf[NT][NP];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -664,44 +689,46 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
       }
       strange = __any(hit != 0);
     }
+    if (!strange) {
 #pragma unroll
-    for (int w = 0; w < VW; ++w) {
-      uint32_t lo[4], hi[4];                                            // bytes {x0, y0, x1, y1} and {x2, y2, x3, y3} of two tokens' dwords
+      for (int w = 0; w < VW; ++w) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo[i] = __builtin_amdgcn_perm(cur.v[2 * i + 1][w], cur.v[2 * i][w], 0x05010400u);
-        hi[i] = __builtin_amdgcn_perm(cur.v[2 * i + 1][w], cur.v[2 * i][w], 0x07030602u);
-      }
+        for (int g = 0; g < VG; ++g) {
+          Frag vf;
+          value_frag<DK>(vf, cur.v, w, g, vsc);
 #pragma unroll
-      for (int g = 0; g < (W < 4 ? W : 4); ++g) {
-        Frag vf;
+          for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t src = g < 2 ? lo[i] : hi[i];
-          vf.h[i] = g & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, cur.vs, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, cur.vs, false);
+            for (int p = NP - 1; p >= 0; --p)
+              o[t][4 * w + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[t][p].v, o[t][4 * w + g], 0, 0, 0);
+          }
         }
-        Frag nan;
-        if (strange) {
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+#pragma unroll
+        for (int g = 0; g < VG; ++g) {
+          Frag vf, nan;
+          value_frag<DK>(vf, cur.v, w, g, vsc);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {                                 // 1 where the value is NaN, and the value 0 there
             const bool n0 = (vf.u[i] & 0x7FFFu) > 0x7F80u, n1 = (vf.u[i] >> 16 & 0x7FFFu) > 0x7F80u;
             nan.u[i] = (n0 ? 0x3F80u : 0u) | (n1 ? 0x3F800000u : 0u);
             vf.u[i] &= (n0 ? 0u : 0xFFFFu) | (n1 ? 0u : 0xFFFF0000u);
           }
-        }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-#pragma unroll
-          for (int p = NP - 1; p >= 0; --p)
-            o[t][4 * w + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[t][p].v, o[t][4 * w + g], 0, 0, 0);
-          if (strange) {
-            Frag see;
+          for (int t = 0; t < NT; ++t) {
+            Frag see;                                                   // 1 where the row sees the token
             const int64_t left = end[t] - (t0 + 8 * quad);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               see.u[i] = (2 * i < left && (seen >> (2 * i) & 1) ? 0x3F80u : 0u) | (2 * i + 1 < left && (seen >> (2 * i + 1) & 1) ? 0x3F800000u : 0u);
             floatx4 cnt = floatx4{0.f, 0.f, 0.f, 0.f};
             cnt = __builtin_amdgcn_mfma_f32_16x16x32_bf16(nan.v, see.v, cnt, 0, 0, 0);
+#pragma unroll
+            for (int p = NP - 1; p >= 0; --p)
+              o[t][4 * w + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[t][p].v, o[t][4 * w + g], 0, 0, 0);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (cnt[e] > 0.f) o[t][4 * w + g][e] = __uint_as_float(0x7FC00000u);
@@ -773,33 +800,56 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
   }
 }
 
-// joins the parts of a split row: one wave a row
+// joins the parts of a split row: a block a row; DK / 4 threads hold four dimensions each, the others take every so-manieth part
 template <typename T>
 __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a, int dk) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.rows) return;
+  __shared__ float w[1024], red[4];
+  __shared__ float4 sums[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x;
   const int g = (int)(row % a.G);
   int64_t rest = row / a.G;
   const int i = (int)(rest % a.Lq);
   rest /= a.Lq;
   const int head = (int)(rest % a.h), b = (int)(rest / a.h);
   const float* ml = a.ws + a.rows * a.splits * dk + row * a.splits * 2;
-  const float* part = a.ws + row * a.splits * dk;
   float M = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) M = fmaxf(M, ml[2 * s]);
+  for (int s = tid; s < a.splits; s += 256) M = fmaxf(M, w[s] = ml[2 * s]);
   M = wave_max(M);
+  if (lane == 0) red[wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float z = M == -INFINITY ? 0.f : M;
   float l = 0.f;
-  for (int s = lane; s < a.splits; s += 64) l += __builtin_amdgcn_exp2f(ml[2 * s] - z) * ml[2 * s + 1];
-  l = wave_sum(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* dst = reinterpret_cast<T*>(a.o) + (int64_t)b * a.ldob + (int64_t)i * a.ldoi + (int64_t)(head * a.G + g) * a.ldoh;
-  for (int d = lane; d < dk; d += 64) {
-    float acc = 0.f;
-    for (int s = 0; s < a.splits; ++s) acc += __builtin_amdgcn_exp2f(ml[2 * s] - z) * part[(int64_t)s * dk + d];
-    Elem<T>::put(dst + d, acc * inv);
+  for (int s = tid; s < a.splits; s += 256) {
+    w[s] = __builtin_amdgcn_exp2f(w[s] - z);
+    l += w[s] * ml[2 * s + 1];
   }
+  l = wave_sum(l);
+  __syncthreads();
+  if (lane == 0) red[wave] = l;
+  __syncthreads();
+  l = (red[0] + red[1]) + (red[2] + red[3]);
+  const int per = dk >> 2, d = tid % per, p0 = tid / per, np = 256 / per;
+  const float4* part = reinterpret_cast<const float4*>(a.ws + row * a.splits * dk) + d;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = p0; s < a.splits; s += np) {
+    const float4 v = part[(size_t)s * per];
+    const float f = w[s];
+    acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+  }
+  sums[tid] = acc;
+  __syncthreads();
+  if (tid >= per) return;
+  for (int k = 1; k < np; ++k) {
+    const float4 v = sums[tid + k * per];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;                           // no visible key: zeros
+  T* dst = reinterpret_cast<T*>(a.o) + (int64_t)b * a.ldob + (int64_t)i * a.ldoi + (int64_t)(head * a.G + g) * a.ldoh + 4 * d;
+  const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  Elem<T>::store4(dst, y);
 }
 
 bool page_ok(int page) { return page >= 16 && page <= 256 && (page & (page - 1)) == 0; }
@@ -813,7 +863,7 @@ int check_cache(const char* who, const uint8_t* kc, const uint8_t* vc, const uin
   TVAE_CHECK(type_bytes(dtype), TVAE_E_DTYPE, "%s: dtype %d is not TVAE_F32, TVAE_BF16 or TVAE_F16", who, dtype);
   TVAE_CHECK(n >= 0 && h > 0 && dk_ok(dk) && page_ok(page), TVAE_E_SHAPE,
              "%s: need n >= 0, h >= 1, dk in {32, 64, 128, 256}, page a power of two in [16, 256] (n=%d h=%d dk=%d page=%d)", who, n, h, dk, page);
-  TVAE_CHECK(n_pages >= 0 && per_seq >= 1 && (int64_t)per_seq * page <= INT32_MAX, TVAE_E_SHAPE,
+  TVAE_CHECK(n_pages >= 1 && per_seq >= 1 && (int64_t)per_seq * page <= INT32_MAX, TVAE_E_SHAPE,
              "%s: bad page counts (n_pages=%d, %d a sequence of %d tokens)", who, n_pages, per_seq, page);
   TVAE_CHECK(table || (int64_t)n * per_seq <= n_pages, TVAE_E_SHAPE, "%s: %d sequences of %d pages do not fit %d pages", who, n, per_seq, n_pages);
   TVAE_CHECK(aligned16(kc) && aligned16(vc), TVAE_E_SHAPE, "%s: cache codes must be 16-byte aligned", who);
@@ -855,7 +905,7 @@ void launch_attn(const AttnArgs& a, int dk, hipStream_t s) {
   else if (dk == 64) launch_dk<T, 64>(a, s);
   else if (dk == 128) launch_dk<T, 128>(a, s);
   else launch_dk<T, 256>(a, s);
-  if (a.splits > 1) hipLaunchKernelGGL((kv8_attn_join_kernel<T>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a, dk);
+  if (a.splits > 1) hipLaunchKernelGGL((kv8_attn_join_kernel<T>), dim3((unsigned)a.rows), dim3(256), 0, s, a, dk);
 }
 
 }  // namespace
@@ -920,11 +970,12 @@ extern "C" int tvae_kv8_attn(const void* q, int64_t ldqb, int64_t ldqi, int64_t 
   TVAE_CHECK(!key_mask || (mask_w >= 0 && ld_mask >= mask_w), TVAE_E_SHAPE, "tvae_kv8_attn: bad mask shape");
   TVAE_CHECK(splits >= 1 && splits <= 1024 && (splits == 1 || ws), TVAE_E_SHAPE, "tvae_kv8_attn: 1 .. 1024 splits, more than one with a workspace");
   const int64_t rows = (int64_t)n * Lq * h * G;
-  TVAE_CHECK((rows + 3) / 4 <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_attn: too many query rows in one call");
+  TVAE_CHECK((splits > 1 ? rows : (rows + 3) / 4) <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_attn: too many query rows in one call");
   if (rows == 0) return TVAE_OK;
   const int64_t cap = lens ? (int64_t)per_seq * page : len0;
   int64_t chunk = ((cap + splits - 1) / splits + 127) / 128 * 128;
   chunk = chunk < INT32_MAX ? chunk : INT32_MAX;
+  if (key_mask && mask_w == 0) { key_mask = ke; ld_mask = 0; }           // no byte of it counts, but one is read
   AttnArgs a = {q, o, ldqb, ldqi, ldqh, ldob, ldoi, ldoh, {kc, vc}, {ke, ve}, {table, per_seq, n_pages}, lens, key_mask, ws, rows,
                 ld_mask, mask_w, len0, causal, n, h, G, Lq, page, splits, (int)chunk, scale * 1.44269504088896341f};
   if (dtype == TVAE_F32) launch_attn<float>(a, dk, (hipStream_t)stream);

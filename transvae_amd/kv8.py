@@ -170,7 +170,7 @@ class KV8Cache:
             self._on(out, "out")
             o = _rows(out, "out")
         if splits is None:
-            splits = self._splits(n * Lq * hq, per * self.page if lp is not None else l0)
+            splits = self._splits(n, hq // self.heads * Lq, per * self.page if lp is not None else l0)
         ws = None
         if splits > 1:
             ws = torch.empty(n * Lq * hq * splits * (dk + 2), dtype=torch.float32, device=q.device)
@@ -181,5 +181,7 @@ class KV8Cache:
             out.copy_(o)
         return out
 
-    def _splits(self, rows, keys):
-        return max(1, min(-(-keys // 512), 2048 // max(1, rows)))
+    def _splits(self, n, rows, keys):
+        "parts for n sequences whose every key head has `rows` query rows"
+        units = n * self.heads * -(-rows // 16)                    # a block of four waves each, and part
+        return max(1, min(-(-keys // 512), 2048 // max(1, units), 1024))
