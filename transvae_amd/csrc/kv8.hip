@@ -489,14 +489,13 @@ struct CodeTile {
   uint32_t k[2][KN];
   uint32_t v[8][VW];
   int ek, ev;                // exponents of the lane's tokens 8 quad .. + 7
-  bool have;                 // their page exists
 
-  // idk, idv: pages of the tokens that the lane loads for the scores and for the second product; -1 reads page 0 instead
-  __device__ inline void load(const AttnArgs& a, int head, int idk, int idv, int64_t t0, int c, int quad) {
+  // id0, id1: pages of the group's first and last 16 tokens (one page unless pages hold 16)
+  __device__ inline void load(const AttnArgs& a, int head, int id0, int id1, int in_page, int c, int quad) {
     const int pm = a.page - 1;
-    have = idv >= 0;
-    const size_t pk = ((size_t)(idk < 0 ? 0 : idk) * a.h + head) * a.page, ph = (size_t)(idv < 0 ? 0 : idv) * a.h + head;
-    const uint8_t* p = a.codes[0] + (pk + ((int)(t0 + 8 * (c >> 2)) & pm) + (c & 3)) * DK;
+    const size_t p0 = (size_t)id0 * a.h + head, p1 = (size_t)id1 * a.h + head;
+    const size_t pk = c >= 8 ? p1 : p0, pv = quad >= 2 ? p1 : p0;
+    const uint8_t* p = a.codes[0] + pk * a.page * DK + (in_page + (8 * (c >> 2) & pm) + (c & 3)) * DK;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint8_t* r = p + 4 * i * DK;
@@ -507,8 +506,8 @@ struct CodeTile {
         for (int w = 0; w < DK / 64; ++w) *reinterpret_cast<uint4*>(k[i] + 4 * w) = *reinterpret_cast<const uint4*>(r + 64 * w + 16 * quad);
       }
     }
-    ek = a.exps[0][ph];
-    p = a.codes[1] + (ph * a.page + ((int)(t0 + 8 * quad) & pm)) * DK + W * c;
+    ek = a.exps[0][pv];
+    p = a.codes[1] + pv * a.page * DK + (in_page + (8 * quad & pm)) * DK + W * c;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (W == 2) v[j][0] = *reinterpret_cast<const uint16_t*>(p + j * DK);
@@ -516,7 +515,7 @@ struct CodeTile {
       else if (W == 8) *reinterpret_cast<uint2*>(v[j]) = *reinterpret_cast<const uint2*>(p + j * DK);
       else *reinterpret_cast<uint4*>(v[j]) = *reinterpret_cast<const uint4*>(p + j * DK);
     }
-    ev = a.exps[1][ph];
+    ev = a.exps[1][pv];
   }
 };
 
@@ -537,11 +536,11 @@ __device__ inline void value_frag(Frag& f, const uint32_t (&v)[8][CodeTile<DK>::
 // score passes it by 2^8: until then weights just exceed 1, which costs no precision and saves the rescaling.
 // KW = 4: the block's waves take every fourth group of 32 tokens and meet at the end; KW = 1: every wave has rows of its own.
 template <typename T, int DK, int NT, int KW>
-__global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv8_attn_tile_kernel(AttnArgs a) {
   constexpr int W = DK / 16, KS = DK / 32, NQ = Pieces<T>::Q, NP = Pieces<T>::P, VW = CodeTile<DK>::VW, VG = W < 4 ? W : 4;
   constexpr int REGS = NT * (4 * W + 2);
   __shared__ float buf[KW == 1 ? 1 : 2 * REGS * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, quad = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, quad = lane >> 4;
   const int M = a.G * a.Lq, mt = (M + 16 * NT - 1) / (16 * NT);
   int64_t unit = KW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   if (unit >= (int64_t)a.n * a.h * mt) return;                          // KW == 4: one unit a block, uniform
@@ -588,22 +587,24 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
 #pragma unroll
     for (int g = 0; g < W; ++g) o[t][g] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  const int shift = 31 - __clz(a.page);
+  const int shift = 31 - __clz(a.page), pm = a.page - 1;
   const PageRow pages(a.pages, b, a.codes[0]);
   const int64_t step = 32 * KW;
   int64_t t0 = beg + 32 * kw;
-  const int ofk = 8 * (c >> 2), ofv = 8 * quad;
   auto ask = [&](int64_t tok) { return pages.ask(tok < most ? (int)(tok >> shift) : 0); };
   auto page = [&](int raw, int64_t tok) { return pages.page(raw, (int)(tok >> shift), tok < most); };
-  // page ids are looked up two groups ahead, codes loaded one group ahead
+  // page ids (the same for all lanes) are looked up two groups ahead, codes loaded one group ahead; where there is no page, page 0
+  // is read instead
   CodeTile<DK> cur, nxt;
-  int rk = ask(t0 + ofk), rv = ask(t0 + ofv);
-  cur.load(a, head, page(rk, t0 + ofk), page(rv, t0 + ofv), t0, c, quad);
-  rk = ask(t0 + step + ofk), rv = ask(t0 + step + ofv);
+  int ra = ask(t0), rb = ask(t0 + 16);
+  int id0 = page(ra, t0), id1 = page(rb, t0 + 16), nd0, nd1;
+  ra = ask(t0 + step), rb = ask(t0 + step + 16);
+  cur.load(a, head, id0 < 0 ? 0 : id0, id1 < 0 ? 0 : id1, (int)t0 & pm, c, quad);
+  bool strange = false;
   for (; t0 < most; t0 += step) {
-    const int idk = page(rk, t0 + step + ofk), idv = page(rv, t0 + step + ofv);
-    rk = ask(t0 + 2 * step + ofk), rv = ask(t0 + 2 * step + ofv);
-    nxt.load(a, head, idk, idv, t0 + step, c, quad);
+    nd0 = page(ra, t0 + step), nd1 = page(rb, t0 + step + 16);
+    ra = ask(t0 + 2 * step), rb = ask(t0 + 2 * step + 16);
+    nxt.load(a, head, nd0 < 0 ? 0 : nd0, nd1 < 0 ? 0 : nd1, (int)(t0 + step) & pm, c, quad);
     // scores: sc[t][i] is the lane's query c of tile t against token t0 + 8 quad + i
     floatx4 sc[NT][2];
 #pragma unroll
@@ -625,10 +626,10 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
         }
       }
     }
-    const bool plain = t0 + 32 <= least && !a.mask && __all(cur.have);  // every row of the unit sees all 32 tokens
+    const bool plain = t0 + 32 <= least && !a.mask && id0 >= 0 && id1 >= 0;      // every row of the unit sees all 32 tokens
     uint32_t seen = 0xFF;                                               // bit i: token 8 quad + i exists and is not masked
     if (!plain) {
-      if (!cur.have) seen = 0;
+      if ((quad >= 2 ? id1 : id0) < 0) seen = 0;
       if (a.mask) {
         const uint8_t* mk = a.mask + (int64_t)b * a.ld_mask;
         uint8_t mb[8];
@@ -641,11 +642,21 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
         for (int i = 0; i < 8; ++i)
           if (t0 + 8 * quad + i >= a.mask_w || mb[i] == 0) seen &= ~(1u << i);
       }
+      // codes that no row sees must not be NaN (0 * NaN is not 0); nor may those that only some rows see: they are taken out
+      // here and put back behind the loop
+      const bool some = least < most && t0 + 32 > least;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {                                     // codes that no row sees: 0 * NaN would not vanish
-        if (!(t0 + 8 * quad + i < most) || !(seen >> i & 1)) {
+      for (int i = 0; i < 8; ++i) {
+        const bool dead = !(t0 + 8 * quad + i < most) || !(seen >> i & 1);
 #pragma unroll
-          for (int w = 0; w < VW; ++w) cur.v[i][w] = 0;
+        for (int w = 0; w < VW; ++w) {
+          uint32_t x = dead ? 0u : cur.v[i][w];
+          if (some) {
+            const uint32_t hit = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+            strange = strange || hit != 0;
+            x &= ~((hit >> 7) * 0xFFu);
+          }
+          cur.v[i][w] = x;
         }
       }
     }
@@ -678,65 +689,39 @@ __global__ __launch_bounds__(256) void kv8_attn_tile_kernel(AttnArgs a) {
       }
       cut_pieces<NP>(x, pf[t]);
     }
-    // a token that some rows see and others do not, whose value is NaN: take it out here and put it back below
-    bool strange = false;
-    if (!plain && least < most && t0 + 32 > least) {
-      uint32_t hit = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+    for (int w = 0; w < VW; ++w) {
 #pragma unroll
-        for (int w = 0; w < VW; ++w) hit |= ((cur.v[i][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-      }
-      strange = __any(hit != 0);
-    }
-    if (!strange) {
+      for (int g = 0; g < VG; ++g) {
+        Frag vf;
+        value_frag<DK>(vf, cur.v, w, g, vsc);
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int g = 0; g < VG; ++g) {
-          Frag vf;
-          value_frag<DK>(vf, cur.v, w, g, vsc);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int p = NP - 1; p >= 0; --p)
-              o[t][4 * w + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[t][p].v, o[t][4 * w + g], 0, 0, 0);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-#pragma unroll
-        for (int g = 0; g < VG; ++g) {
-          Frag vf, nan;
-          value_frag<DK>(vf, cur.v, w, g, vsc);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {                                 // 1 where the value is NaN, and the value 0 there
-            const bool n0 = (vf.u[i] & 0x7FFFu) > 0x7F80u, n1 = (vf.u[i] >> 16 & 0x7FFFu) > 0x7F80u;
-            nan.u[i] = (n0 ? 0x3F80u : 0u) | (n1 ? 0x3F800000u : 0u);
-            vf.u[i] &= (n0 ? 0u : 0xFFFFu) | (n1 ? 0u : 0xFFFF0000u);
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            Frag see;                                                   // 1 where the row sees the token
-            const int64_t left = end[t] - (t0 + 8 * quad);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              see.u[i] = (2 * i < left && (seen >> (2 * i) & 1) ? 0x3F80u : 0u) | (2 * i + 1 < left && (seen >> (2 * i + 1) & 1) ? 0x3F800000u : 0u);
-            floatx4 cnt = floatx4{0.f, 0.f, 0.f, 0.f};
-            cnt = __builtin_amdgcn_mfma_f32_16x16x32_bf16(nan.v, see.v, cnt, 0, 0, 0);
-#pragma unroll
-            for (int p = NP - 1; p >= 0; --p)
-              o[t][4 * w + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[t][p].v, o[t][4 * w + g], 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (cnt[e] > 0.f) o[t][4 * w + g][e] = __uint_as_float(0x7FC00000u);
-          }
+          for (int p = NP - 1; p >= 0; --p)
+            o[t][4 * w + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.v, pf[t][p].v, o[t][4 * w + g], 0, 0, 0);
         }
       }
     }
+    id0 = nd0, id1 = nd1;
     cur = nxt;
+  }
+  if (__any(strange)) {                                                 // NaN for the rows that see it: token by token, rare
+    for (int64_t g0 = beg + 32 * kw; g0 < most; g0 += step) {
+      if (g0 + 32 <= least) continue;
+      for (int64_t j = g0; j < g0 + 32 && j < most; ++j) {
+        const int id = page(ask(j), j);
+        if (id < 0 || (a.mask && (j >= a.mask_w || a.mask[(int64_t)b * a.ld_mask + j] == 0))) continue;
+        const uint8_t* p = a.codes[1] + (((size_t)id * a.h + head) * a.page + ((int)j & pm)) * DK + 4 * W * quad;
+#pragma unroll
+        for (int i = 0; i < 4 * W; ++i) {                               // dimension W e + g of the lane's 4 W
+          const bool nan = (p[i] & 0x7F) == 0x7F;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            if (nan && j < end[t]) o[t][i % W][i / W] = __uint_as_float(0x7FC00000u);
+        }
+      }
+    }
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) l[t] = quad_sum(l[t]);
