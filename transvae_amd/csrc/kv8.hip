@@ -10,6 +10,7 @@
 #include "common.h"
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 namespace {
 
@@ -18,6 +19,31 @@ constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;              // of 256 threads: a 
 
 struct F16 { _Float16 v; };
 struct B16 { uint16_t v; };
+
+// 16 bytes of a row as they are, and as floats
+template <typename T> struct Raw {
+  static constexpr int N = 16 / sizeof(T);
+  uint4 w;
+  __device__ inline void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ inline void zero() { w = make_uint4(0, 0, 0, 0); }
+  __device__ inline void values(float (&x)[N]) const;
+  // what was unpacked from w so far is not kept: a second look unpacks again instead of holding 8 registers for 4
+  __device__ inline void forget() { asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w)); }
+};
+template <> __device__ inline void Raw<float>::values(float (&x)[4]) const {
+  x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
+}
+template <> __device__ inline void Raw<B16>::values(float (&x)[8]) const {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(u[i] << 16); x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u); }
+}
+template <> __device__ inline void Raw<F16>::values(float (&x)[8]) const {
+  _Float16 h[8];
+  *reinterpret_cast<uint4*>(h) = w;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+}
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -61,26 +87,37 @@ template <> struct Elem<F16> {
 __device__ inline float exp_scale(int e) { return __uint_as_float((uint32_t)e << 23); }          // 2^(e - 127)
 __device__ inline float inv_scale(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }  // 2^(127 - e)
 
+// Magnitudes are compared as whole numbers (the bits without the sign): one comparison also finds infinities and NaN, which
+// are rare enough for a second look.
+constexpr uint32_t INF_BITS = 0x7F800000u;
+__device__ inline uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+__device__ inline uint32_t finite_magnitude(float x) {
+  const uint32_t u = magnitude(x);
+  return u < INF_BITS ? u : 0u;
+}
 // stored exponent for a largest magnitude (448 = 1.75 * 2^8: a mantissa above 1.75 carries into the exponent)
-__device__ inline int need_exp(float amax) {
-  const int e = (int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 8;
+__device__ inline int need_exp(uint32_t top) {
+  const int e = (int)((top + 0x1FFFFFu) >> 23) - 8;
   return e < E_MIN ? E_MIN : e > E_MAX ? E_MAX : e;
-}
-__device__ inline float finite_abs(float x) {
-  const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
-  return u < 0x7F800000u ? __uint_as_float(u) : 0.f;
-}
-// e4m3 operand of a value: scaled and clamped (the largest exponent cannot hold every float), non-finite -> NaN (the format
-// has no infinity, and a saturated one would read back as an ordinary number)
-__device__ inline float to_range(float x, float inv) {
-  const float y = fminf(fmaxf(x * inv, -448.f), 448.f);
-  return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u ? __uint_as_float(0x7FC00000u) : y;
 }
 __device__ inline uint32_t pack4(const float (&y)[4]) {
   uint32_t w = 0;
   w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], w, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
   return w;
+}
+// codes of four values.  `odd`: the page's rows hold a non-finite value (NaN is stored: the format has no infinity, and a saturated
+// one would read back as an ordinary number) or take the largest exponent (which cannot hold every float: those saturate).
+// Otherwise the scale itself keeps every value within +-448.
+__device__ inline uint32_t encode4(const float (&x)[4], float inv, bool odd) {
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = x[i] * inv;
+  if (odd) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = magnitude(x[i]) >= INF_BITS ? __uint_as_float(0x7FC00000u) : fminf(fmaxf(y[i], -448.f), 448.f);
+  }
+  return pack4(y);
 }
 __device__ inline void unpack4(uint32_t w, float (&x)[4]) {
   const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
@@ -112,6 +149,39 @@ struct PageRow {
   }
 };
 
+template <int CTRL> __device__ inline float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+// sum / maximum over groups of N neighbouring lanes (every lane of a group gets it): quad permutes, mirrors of 8 and 16, then swaps
+template <int N> __device__ inline float group_sum(float x) {
+  if (N >= 2) x += dpp<0xB1>(x);
+  if (N >= 4) x += dpp<0x4E>(x);
+  if (N >= 8) x += dpp<0x141>(x);
+  if (N >= 16) x += dpp<0x140>(x);
+  return x;
+}
+template <int CTRL> __device__ inline uint32_t dpp(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true); }
+template <int N> __device__ inline uint32_t group_max(uint32_t x) {
+  if (N >= 2) x = max(x, dpp<0xB1>(x));
+  if (N >= 4) x = max(x, dpp<0x4E>(x));
+  if (N >= 8) x = max(x, dpp<0x141>(x));
+  if (N >= 16) x = max(x, dpp<0x140>(x));
+  if (N >= 32) x = max(x, (uint32_t)__shfl_xor((int)x, 16, 64));
+  if (N >= 64) x = max(x, (uint32_t)__shfl_xor((int)x, 32, 64));
+  return x;
+}
+
+// x / d for x < 2^31 and a divisor that the host knows: with 2^(s-1) < d <= 2^s, m = ceil(2^(31+s) / d) fits 32 bits and
+// (x m) >> (31 + s) is exact (m exceeds 2^(31+s) / d by less than 1, x times that is less than 2^31 <= 2^(31+s) / d)
+struct Divisor {
+  uint32_t d, m, s;
+  explicit Divisor(uint32_t by) : d(by), m(0), s(0) {
+    while ((1u << s) < by) ++s;
+    m = (uint32_t)((((uint64_t)1 << (31 + s)) + by - 1) / by);
+  }
+  __device__ inline uint32_t div(uint32_t x) const { return (uint32_t)(((uint64_t)x * m) >> (31 + s)); }
+};
+
 // ------------------------------------------------------------------------------------------------ store
 struct StoreArgs {
   const void* src[2];
@@ -121,75 +191,193 @@ struct StoreArgs {
   Pages pages;
   const int32_t* start;
   const int32_t* count;
-  int start0, n, T, h, dk, page, slots;
+  Divisor by_h;
+  int start0, n, T, h, page, slots;
 };
 
-// One wave per (sequence, touched page, head, K or V): the largest magnitude of the new rows, the page's exponent, then the
-// codes.  Rows in front of the new ones are only rewritten when the exponent grows.
-template <typename T>
-__global__ __launch_bounds__(256) void kv8_store_kernel(StoreArgs a) {
-  const int lane = threadIdx.x & 63;
-  int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int side = (int)(unit & 1);
-  unit >>= 1;
-  const int head = (int)(unit % a.h);
-  unit /= a.h;
-  const int slot = (int)(unit % a.slots), b = (int)(unit / a.slots);
-  if (b >= a.n) return;
+// the rows in front of the new ones, from their old scale to a larger one: each value is rounded again; N codes a lane
+template <int N>
+__device__ inline void rescale_rows(uint8_t* dst, int r0, int dk, int step, int old, int e) {
+  int d = old - e;
+  d = d > -40 ? d : -40;                                                // beyond that everything rounds to zero
+  const float f = exp_scale(E_BIAS + d);
+  for (int i = 0; i < r0; i += step) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(dst + (size_t)i * dk);
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      float x[4];
+      unpack4(w[j], x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] *= f;
+      w[j] = pack4(x);
+    }
+  }
+}
+
+template <typename T> __device__ inline uint32_t top_of(const Raw<T>& r, bool strange) {
+  float x[Raw<T>::N];
+  r.values(x);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < Raw<T>::N; ++i) top = max(top, strange ? finite_magnitude(x[i]) : magnitude(x[i]));
+  return top;
+}
+template <typename T> __device__ inline void put_codes(uint8_t* dst, const Raw<T>& r, float inv, bool odd) {
+  float x[Raw<T>::N];
+  r.values(x);
+  uint32_t w[Raw<T>::N / 4];
+#pragma unroll
+  for (int i = 0; i < Raw<T>::N; i += 4) {
+    const float y[4] = {x[i], x[i + 1], x[i + 2], x[i + 3]};
+    w[i / 4] = encode4(y, inv, odd);
+  }
+  if (Raw<T>::N == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+  else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[Raw<T>::N / 4 - 1]);
+}
+
+// A few rows a sequence (T <= 4: a decode step, drafted tokens).  The lanes that one row's 16-byte pieces take hold the K and
+// the V rows of one (sequence, head) in registers: their maxima, the page's exponents, the codes.  Bound by latency more than
+// by the rows' bytes, hence both sides in one thread.
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void kv8_append_kernel(StoreArgs a) {
+  constexpr int N = Raw<T>::N, LPR = DK / N;
+  const int sub = threadIdx.x % LPR;
+  const uint32_t unit = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (unit >= (uint32_t)a.n * a.h) return;
+  const int b = (int)a.by_h.div(unit), head = (int)unit - b * a.h;
   const int64_t beg = a.start ? a.start[b] : a.start0;
   int cnt = a.count ? a.count[b] : a.T;
   cnt = cnt < a.T ? cnt : a.T;
   if (beg < 0 || cnt <= 0) return;
-  const int64_t pslot = beg / a.page + slot;
+  Raw<T> x[2][4];
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const T* src = reinterpret_cast<const T*>(a.src[side]) + (int64_t)b * a.ldb[side] + (int64_t)head * a.ldh[side] + N * sub;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (t < cnt) x[side][t].load(src + t * a.ldt[side]);
+      else x[side][t].zero();
+    }
+  }
+  const int shift = 31 - __clz(a.page);
+  for (int t0 = 0; t0 < cnt;) {                                         // page after page: two at most
+    const int64_t slot = (beg + t0) >> shift;
+    if (slot >= a.pages.per_seq) return;
+    const int r0 = (int)((beg + t0) & (a.page - 1)), t1 = cnt - t0 < a.page - r0 ? cnt : t0 + a.page - r0;
+    const int id = a.pages.at(b, (int)slot);
+    if (id >= 0) {
+      const size_t ph = (size_t)id * a.h + head;
+      int old[2];
+#pragma unroll
+      for (int side = 0; side < 2; ++side) old[side] = r0 > 0 ? a.exps[side][ph] : 0;
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        uint8_t* dst = a.codes[side] + ph * a.page * DK + N * sub;
+        uint32_t top = 0;
+        bool strange = false;
+        for (int look = 0; look < 2; ++look) {                          // a second time only where something is not finite
+          top = 0;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if (t >= t0 && t < t1) top = max(top, top_of(x[side][t], strange));
+            x[side][t].forget();
+          }
+          top = group_max<LPR>(top);
+          if (top < INF_BITS) break;
+          strange = true;
+        }
+        int e = need_exp(top);
+        if (old[side] >= e) e = old[side] < E_MAX ? old[side] : E_MAX;
+        else if (r0 > 0) rescale_rows<N>(dst, r0, DK, 1, old[side], e);
+        const float inv = inv_scale(e);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (t >= t0 && t < t1) put_codes(dst + (size_t)(r0 + t - t0) * DK, x[side][t], inv, strange || e == E_MAX);
+        if (sub == 0) a.exps[side][ph] = (uint8_t)e;
+      }
+    }
+    t0 = t1;
+  }
+}
+
+// Many rows a sequence: TPU threads per (sequence, touched page, head), K or V.  A thread keeps its first KEEP 16-byte pieces in
+// registers as they came, so the rows are read once; a wave a page where that suffices, a block of four else.
+template <typename T, int DK, int TPU>
+__global__ __launch_bounds__(256) void kv8_store_kernel(StoreArgs a) {
+  constexpr int N = Raw<T>::N, LPR = DK / N, RPI = TPU / LPR, KEEP = 16;        // values a piece, lanes a row, rows a step
+  __shared__ uint32_t red[4];
+  const int tid = threadIdx.x % TPU, side = blockIdx.y;
+  uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * (256 / TPU) + threadIdx.x / TPU);
+  const int head = (int)(unit % a.h);
+  unit /= a.h;
+  const int slot = (int)(unit % a.slots), b = (int)(unit / a.slots);
+  if (b >= a.n) return;                                                 // whole units leave: a block of one unit leaves together
+  const int64_t beg = a.start ? a.start[b] : a.start0;
+  int cnt = a.count ? a.count[b] : a.T;
+  cnt = cnt < a.T ? cnt : a.T;
+  if (beg < 0 || cnt <= 0) return;
+  const int shift = 31 - __clz(a.page);
+  const int64_t pslot = (beg >> shift) + slot;
   if (pslot >= a.pages.per_seq) return;
-  const int64_t p0 = pslot * a.page;                                     // first position of the page
-  const int r0 = (int)(beg > p0 ? beg - p0 : 0);                         // rows [r0, r1) of the page are new
+  const int64_t p0 = pslot << shift;                                    // first position of the page
+  const int r0 = (int)(beg > p0 ? beg - p0 : 0);                        // rows [r0, r1) of the page are new
   const int64_t left = beg + cnt - p0;
   const int r1 = (int)(left < a.page ? left : a.page);
   if (r0 >= r1) return;
   const int id = a.pages.at(b, (int)pslot);
   if (id < 0) return;
-  const int lpr = a.dk >> 2, sub = lane % lpr, rg = lane / lpr, rpi = 64 / lpr;   // lanes per row, 4 values each
-  const T* src = reinterpret_cast<const T*>(a.src[side]) + (int64_t)b * a.ldb[side] + (int64_t)head * a.ldh[side] + 4 * sub;
-  const int64_t t0 = p0 - beg;
-  float amax = 0.f;
-  for (int r = r0 + rg; r < r1; r += rpi) {
-    float x[4];
-    Elem<T>::load4(src + (t0 + r) * a.ldt[side], x);
+  const int sub = tid % LPR, rg = tid / LPR;
+  const T* src = reinterpret_cast<const T*>(a.src[side]) + (int64_t)b * a.ldb[side] + (int64_t)head * a.ldh[side] + N * sub + (p0 - beg) * a.ldt[side];
+  const size_t ph = (size_t)id * a.h + head;
+  uint8_t* dst = a.codes[side] + ph * a.page * DK + N * sub;
+  const int old = r0 > 0 ? a.exps[side][ph] : 0;
+  Raw<T> x[KEEP];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, finite_abs(x[i]));
+  for (int k = 0; k < KEEP; ++k) {
+    const int r = r0 + rg + k * RPI;
+    if (r < r1) x[k].load(src + r * a.ldt[side]);
+    else x[k].zero();
   }
-  amax = wave_max(amax);
-  uint8_t* ep = a.exps[side] + (size_t)id * a.h + head;
-  uint8_t* dst = a.codes[side] + ((size_t)id * a.h + head) * a.page * a.dk + 4 * sub;
-  int e = need_exp(amax);
-  if (r0 > 0) {
-    const int old = *ep;
-    if (old >= e) {
-      e = old < E_MAX ? old : E_MAX;
-    } else {
-      int d = old - e;
-      d = d > -40 ? d : -40;                                            // beyond that everything rounds to zero
-      const float f = exp_scale(E_BIAS + d);
-      for (int r = rg; r < r0; r += rpi) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(dst + (size_t)r * a.dk);
-        float x[4];
-        unpack4(*w, x);
+  uint32_t top = 0;
+  bool strange = false;
+  for (int look = 0; look < 2; ++look) {                                // a second time only where something is not finite
+    top = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= f;
-        *w = pack4(x);
-      }
+    for (int k = 0; k < KEEP; ++k) {
+      top = max(top, top_of(x[k], strange));
+      x[k].forget();
     }
+    for (int r = r0 + rg + KEEP * RPI; r < r1; r += RPI) {
+      Raw<T> y;
+      y.load(src + r * a.ldt[side]);
+      top = max(top, top_of(y, strange));
+    }
+    top = group_max<64>(top);
+    if (TPU == 256) {
+      __syncthreads();                                                  // also: every thread has read the old exponent
+      if ((tid & 63) == 0) red[tid >> 6] = top;
+      __syncthreads();
+      top = max(max(red[0], red[1]), max(red[2], red[3]));
+    }
+    if (top < INF_BITS) break;
+    strange = true;
   }
+  int e = need_exp(top);
+  if (old >= e) e = old < E_MAX ? old : E_MAX;
+  else if (rg < r0) rescale_rows<N>(dst + (size_t)rg * DK, r0 - rg, DK, RPI, old, e);
   const float inv = inv_scale(e);
-  for (int r = r0 + rg; r < r1; r += rpi) {
-    float x[4];
-    Elem<T>::load4(src + (t0 + r) * a.ldt[side], x);
+  const bool odd = strange || e == E_MAX;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = to_range(x[i], inv);
-    *reinterpret_cast<uint32_t*>(dst + (size_t)r * a.dk) = pack4(x);
+  for (int k = 0; k < KEEP; ++k) {
+    const int r = r0 + rg + k * RPI;
+    if (r < r1) put_codes(dst + (size_t)r * DK, x[k], inv, odd);
   }
-  if (lane == 0) *ep = (uint8_t)e;
+  for (int r = r0 + rg + KEEP * RPI; r < r1; r += RPI) {
+    Raw<T> y;
+    y.load(src + r * a.ldt[side]);
+    put_codes(dst + (size_t)r * DK, y, inv, odd);
+  }
+  if (tid == 0) a.exps[side][ph] = (uint8_t)e;
 }
 
 // ------------------------------------------------------------------------------------------------ load
@@ -200,39 +388,66 @@ struct LoadArgs {
   Pages pages;
   const int32_t* start;
   const int32_t* count;
-  int start0, n, T, h, dk, page;
+  Divisor by_T, by_h;
+  uint32_t total;
+  int start0, T, h, page;
 };
 
-// One thread per 4 values.
-template <typename T>
+// A thread makes four times 16 bytes of the result (4 or 8 values), a block's width apart and all in flight together; tokens of
+// one head lie next to each other: a page's rows of a head are read in order, and what a wave writes are whole rows.  The
+// result is written past the caches: kept in them it only delays the end of the launch (measured at 500 x 127 x 4 x 64 fp32:
+// 40 us through the caches, 27 us past them).
+template <typename T, int DK>
 __global__ __launch_bounds__(256) void kv8_load_kernel(LoadArgs a) {
+  constexpr int N = 16 / sizeof(T), LPR = DK / N, U = 4;
   const int side = blockIdx.y;
-  const int lpr = a.dk >> 2;
-  const int64_t total = (int64_t)a.n * a.h * a.T * lpr;
-  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const int sub = (int)(i % lpr);
-  i /= lpr;
-  const int t = (int)(i % a.T);
-  i /= a.T;
-  const int head = (int)(i % a.h), b = (int)(i / a.h);
-  const int64_t beg = a.start ? a.start[b] : a.start0;
-  int cnt = a.count ? a.count[b] : a.T;
-  const int64_t pos = beg + t;
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (t < cnt && pos >= 0 && pos < (int64_t)a.pages.per_seq * a.page) {
-    const int id = a.pages.at(b, (int)(pos / a.page));
-    if (id >= 0) {
-      const size_t ph = (size_t)id * a.h + head;
-      unpack4(*reinterpret_cast<const uint32_t*>(a.codes[side] + (ph * a.page + pos % a.page) * a.dk + 4 * sub), x);
-      const float s = exp_scale(a.exps[side][ph]);
+  const int shift = 31 - __clz(a.page);
+  const uint32_t i0 = blockIdx.x * (256 * U) + threadIdx.x;
+  int id[U];
+  uint32_t b[U], head[U], t[U], sub[U];
+  int64_t pos[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= s;
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = i0 + 256 * u < a.total ? i0 + 256 * u : 0;
+    const uint32_t row = i / LPR, bh = a.by_T.div(row);
+    sub[u] = i % LPR;
+    t[u] = row - bh * a.T;
+    b[u] = a.by_h.div(bh);
+    head[u] = bh - b[u] * a.h;
+    pos[u] = (int64_t)(a.start ? a.start[b[u]] : a.start0) + t[u];
+    const int cnt = a.count ? a.count[b[u]] : a.T;
+    const bool live = (int)t[u] < cnt && pos[u] >= 0 && (pos[u] >> shift) < a.pages.per_seq;
+    id[u] = live ? a.pages.at((int)b[u], (int)(pos[u] >> shift)) : -1;
+  }
+  uint32_t w[U][N / 4];
+  int e[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const size_t ph = (size_t)(id[u] < 0 ? 0 : id[u]) * a.h + head[u];
+    const uint8_t* p = a.codes[side] + (ph * a.page + ((int)pos[u] & (a.page - 1))) * DK + N * sub[u];
+    w[u][0] = w[u][N / 4 - 1] = 0;
+    e[u] = E_BIAS;
+    if (id[u] >= 0) {
+      if (N == 4) w[u][0] = *reinterpret_cast<const uint32_t*>(p);
+      else *reinterpret_cast<uint2*>(w[u]) = *reinterpret_cast<const uint2*>(p);
+      e[u] = a.exps[side][ph];
     }
   }
-  T* o = reinterpret_cast<T*>(a.out[side]) + (((int64_t)b * a.T + t) * a.h + head) * a.dk + 4 * sub;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) Elem<T>::put(o + e, x[e]);
+  for (int u = 0; u < U; ++u) {
+    if (i0 + 256 * u >= a.total) continue;
+    const float s = exp_scale(e[u]);
+    T out[N];
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      float y[4];
+      unpack4(w[u][k / 4], y);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) Elem<T>::put(out + k + v, y[v] * s);
+    }
+    T* o = reinterpret_cast<T*>(a.out[side]) + (((size_t)b[u] * a.T + t[u]) * a.h + head[u]) * DK + N * sub[u];
+    __builtin_nontemporal_store(*reinterpret_cast<const uintx4*>(out), reinterpret_cast<uintx4*>(o));
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ attend
@@ -250,18 +465,6 @@ struct AttnArgs {
   int mask_w, len0, causal, n, h, G, Lq, page, splits, chunk;
   float scale;               // of the scores, times log2(e)
 };
-
-template <int CTRL> __device__ inline float dpp(float x) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
-}
-// sum over groups of N neighbouring lanes (every lane of a group gets it): quad permutes, then mirrors of 8 and of 16
-template <int N> __device__ inline float group_sum(float x) {
-  if (N >= 2) x += dpp<0xB1>(x);
-  if (N >= 4) x += dpp<0x4E>(x);
-  if (N >= 8) x += dpp<0x141>(x);
-  if (N >= 16) x += dpp<0x140>(x);
-  return x;
-}
 
 __device__ inline int seq_len(const AttnArgs& a, int b) {
   int64_t len = a.lens ? a.lens[b] : a.len0;
@@ -860,6 +1063,28 @@ bool rows_ok(const void* p, int64_t ldb, int64_t ldt, int64_t ldh, int dtype) {
 }
 
 template <typename T, int DK>
+void launch_store_dk(const StoreArgs& a, int units, hipStream_t s) {
+  constexpr int N = Raw<T>::N;
+  if (a.T <= 4) hipLaunchKernelGGL((kv8_append_kernel<T, DK>), dim3(cdiv(units, 256 * N / DK)), dim3(256), 0, s, a);
+  else if (a.page * DK <= 64 * 16 * N) hipLaunchKernelGGL((kv8_store_kernel<T, DK, 64>), dim3(cdiv(units, 4), 2), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((kv8_store_kernel<T, DK, 256>), dim3(units, 2), dim3(256), 0, s, a);
+}
+template <typename T>
+void launch_store(const StoreArgs& a, int dk, int units, hipStream_t s) {
+  if (dk == 32) launch_store_dk<T, 32>(a, units, s);
+  else if (dk == 64) launch_store_dk<T, 64>(a, units, s);
+  else if (dk == 128) launch_store_dk<T, 128>(a, units, s);
+  else launch_store_dk<T, 256>(a, units, s);
+}
+template <typename T>
+void launch_load(const LoadArgs& a, int dk, hipStream_t s) {
+  const dim3 grid((a.total + 1023) / 1024, 2);
+  if (dk == 32) hipLaunchKernelGGL((kv8_load_kernel<T, 32>), grid, dim3(256), 0, s, a);
+  else if (dk == 64) hipLaunchKernelGGL((kv8_load_kernel<T, 64>), grid, dim3(256), 0, s, a);
+  else if (dk == 128) hipLaunchKernelGGL((kv8_load_kernel<T, 128>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((kv8_load_kernel<T, 256>), grid, dim3(256), 0, s, a);
+}
+template <typename T, int DK>
 void launch_row(const AttnArgs& a, hipStream_t s) {
   if (a.rows * a.splits >= 8192)
     hipLaunchKernelGGL((kv8_attn_row_kernel<T, DK, 1>), dim3((unsigned)((a.rows + 3) / 4), a.splits), dim3(256), 0, s, a);
@@ -908,14 +1133,13 @@ extern "C" int tvae_kv8_store(const void* k, int64_t ldkb, int64_t ldkt, int64_t
              "tvae_kv8_store: k and v rows must be 16-byte aligned");
   if (n == 0 || T == 0) return TVAE_OK;
   const int slots = (T - 1 + page - 1) / page + 1;                      // pages that T rows can touch
-  const int64_t units = (int64_t)n * slots * h * 2;
-  TVAE_CHECK((units + 3) / 4 <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_store: too many pages in one call");
+  const int64_t units = T <= 4 ? (int64_t)n * h : (int64_t)n * slots * h;
+  TVAE_CHECK(units <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_store: too many pages in one call");
   StoreArgs a = {{k, v}, {ldkb, ldvb}, {ldkt, ldvt}, {ldkh, ldvh}, {kc, vc}, {ke, ve}, {table, per_seq, n_pages}, start, count,
-                 start0, n, T, h, dk, page, slots};
-  const dim3 grid((unsigned)((units + 3) / 4));
-  if (dtype == TVAE_F32) hipLaunchKernelGGL(kv8_store_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else if (dtype == TVAE_BF16) hipLaunchKernelGGL(kv8_store_kernel<B16>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL(kv8_store_kernel<F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+                 Divisor(h), start0, n, T, h, page, slots};
+  if (dtype == TVAE_F32) launch_store<float>(a, dk, (int)units, (hipStream_t)stream);
+  else if (dtype == TVAE_BF16) launch_store<B16>(a, dk, (int)units, (hipStream_t)stream);
+  else launch_store<F16>(a, dk, (int)units, (hipStream_t)stream);
   TVAE_LAUNCH_CHECK("tvae_kv8_store");
   return TVAE_OK;
 }
@@ -928,13 +1152,12 @@ extern "C" int tvae_kv8_load(const uint8_t* kc, const uint8_t* vc, const uint8_t
   if (rc) return rc;
   TVAE_CHECK(T >= 0 && aligned16(k) && aligned16(v), TVAE_E_SHAPE, "tvae_kv8_load: T must not be negative, k and v 16-byte aligned");
   if (n == 0 || T == 0) return TVAE_OK;
-  const int64_t blocks = ((int64_t)n * h * T * (dk / 4) + 255) / 256;
-  TVAE_CHECK(blocks <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_load: too many rows in one call");
-  LoadArgs a = {{kc, vc}, {ke, ve}, {k, v}, {table, per_seq, n_pages}, start, count, start0, n, T, h, dk, page};
-  const dim3 grid((unsigned)blocks, 2);
-  if (dtype == TVAE_F32) hipLaunchKernelGGL(kv8_load_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else if (dtype == TVAE_BF16) hipLaunchKernelGGL(kv8_load_kernel<B16>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL(kv8_load_kernel<F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  const int64_t total = (int64_t)n * h * T * (dk * type_bytes(dtype) / 16);
+  TVAE_CHECK((int64_t)n * h <= INT32_MAX && total <= INT32_MAX, TVAE_E_SHAPE, "tvae_kv8_load: too many rows in one call");
+  LoadArgs a = {{kc, vc}, {ke, ve}, {k, v}, {table, per_seq, n_pages}, start, count, Divisor(T), Divisor(h), (uint32_t)total, start0, T, h, page};
+  if (dtype == TVAE_F32) launch_load<float>(a, dk, (hipStream_t)stream);
+  else if (dtype == TVAE_BF16) launch_load<B16>(a, dk, (hipStream_t)stream);
+  else launch_load<F16>(a, dk, (hipStream_t)stream);
   TVAE_LAUNCH_CHECK("tvae_kv8_load");
   return TVAE_OK;
 }
