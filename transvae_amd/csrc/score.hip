@@ -54,6 +54,13 @@ struct Sums {
     l += e;
     t = fmaf(e, fmaxf(d, -1e30f), t);                      // -inf adds 0, not 0 * inf
   }
+  __device__ inline void over_wave() {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), t2 = __shfl_xor(t, o, 64);
+      join(m2, l2, t2);
+    }
+  }
   __device__ inline void join(float m2, float l2, float t2) {
     if (m2 > m) grow(m2);
     if (l2 != 0.f) {
@@ -64,17 +71,36 @@ struct Sums {
   }
 };
 
-struct TopList {                                           // lane i < top holds the i-th best
-  int key = NO_KEY, idx = 0, last = NO_KEY;                // last: key of entry top - 1, the same in all lanes
+template <int CTRL> __device__ inline int dpp(int x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false); }
+
+// A wave's best: lane i < top holds the i-th (by descending key, then ascending class).
+struct TopList {
+  int key = NO_KEY, idx = INT32_MAX;
+  int last = NO_KEY;                                       // key of entry top - 1, the same in all lanes
   float bar = __int_as_float(0x7FC00000);                  // its value; NaN while the list is not full: nothing is <= NaN
-  __device__ inline void insert(int k, int i, int lane, int top) {      // k, i uniform; values come in ascending order of i
-    if (k <= last) return;
-    const int pos = __popcll(__ballot(lane < top && key >= k));
-    const int ku = __shfl_up(key, 1, 64), iu = __shfl_up(idx, 1, 64);
+  __device__ inline void insert(int k, int i, int lane, int top) {      // k, i uniform
+    const int pos = __popcll(__ballot(lane < top && (key > k || (key == k && idx < i))));
+    if (pos >= top) return;
+    const int ku = dpp<0x138>(key), iu = dpp<0x138>(idx);  // one lane up (wave_shr:1)
     if (lane > pos) { key = ku; idx = iu; }
     if (lane == pos) { key = k; idx = i; }
     last = __builtin_amdgcn_readlane(key, top - 1);
     bar = last == NO_KEY ? __int_as_float(0x7FC00000) : of_key(last);
+  }
+  // A bar before the list has one: the top-th largest of the lanes' own maxima.  That many values reach it, so nothing below
+  // it can be among the best.
+  static __device__ inline float opening_bar(float vm, int lane, int top) {
+    int k = key_of(vm);
+#pragma unroll
+    for (int size = 2; size <= 64; size <<= 1) {           // a bitonic sort across the lanes, descending
+#pragma unroll
+      for (int d = size >> 1; d > 0; d >>= 1) {
+        const int other = __shfl_xor(k, d, 64);
+        const bool up = (lane & size) != 0, low = (lane & d) == 0;
+        k = (low != up) ? max(k, other) : min(k, other);
+      }
+    }
+    return of_key(__builtin_amdgcn_readlane(k, top - 1));
   }
 };
 
@@ -99,8 +125,10 @@ __device__ inline void finish_row(const ScoreArgs& a, int64_t row, const Sums& s
     if (s.l != s.l && y >= 0 && y < a.V) lp = s.l;
     a.logp[row * a.ld_logp] = lp;
     a.entropy[row * a.ld_ent] = none ? 0.f : L - s.t / s.l;
-    a.stat[2 * row] = s.m;
-    a.stat[2 * row + 1] = L;
+    if (a.stat) {
+      a.stat[2 * row] = s.m;
+      a.stat[2 * row + 1] = L;
+    }
   }
   for (int c = tid; c < n; c += threads) {
     const int2 me = cand[c];
@@ -133,23 +161,41 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
     int64_t head = ((16 - ((uintptr_t)(x + c0) & 15)) & 15) / sizeof(T);              // values up to a 16-byte border
     if (head > c1 - c0) head = c1 - c0;
     const int64_t body = (c1 - c0 - head) / NV, tail = c0 + head + body * NV;
-    auto single = [&](int64_t c, bool in) {                // one value a lane
-      const float v = in ? value_of(x[c]) : -INFINITY;
-      if (in) {
-        if (v > s.m) s.grow(v);
-        s.add(v);
-      }
-      if (a.top) {
-        uint64_t todo = __ballot(in);
+    // enters what of v[0 .. N) (lane o's values are classes base + o * N ..) is above the bar that stood before this step; all
+    // earlier entries are lower classes, so equal values behind them stay out, and equal values of one step are told apart
+    // by their class
+    bool first = true;
+    auto enter = [&](auto& v, float vm, bool in, int base) {
+      constexpr int N = sizeof(v) / sizeof(float);
+      const bool opening = first;
+      const float bar = opening ? TopList::opening_bar(in ? vm : -INFINITY, lane, a.top) : top.bar;
+      first = false;
+      const bool odd = s.l != s.l;                         // a NaN went by: the maximum may have passed over it
+      if (!__any(in && (odd || (opening ? !(vm < bar) : !(vm <= bar))))) return;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        uint64_t todo = __ballot(in && (opening ? !(v[e] < bar) : !(v[e] <= bar)));
+        if (!todo) continue;
+        const int k = key_of(v[e]);
         while (todo) {
           const int o = __ffsll((unsigned long long)todo) - 1;
           todo &= todo - 1;
-          top.insert(__builtin_amdgcn_readlane(key_of(v), o), (int)__builtin_amdgcn_readlane((int)c, o), lane, a.top);
+          top.insert(__builtin_amdgcn_readlane(k, o), base + o * N + e, lane, a.top);
         }
       }
     };
-    if (kw == 0 && head) single(c0 + lane, lane < head);
+    auto single = [&](int64_t c0, int n) {                 // one value a lane
+      const bool in = lane < n;
+      float v[1] = {in ? value_of(x[c0 + lane]) : -INFINITY};
+      if (in) {
+        if (v[0] > s.m) s.grow(v[0]);
+        s.add(v[0]);
+      }
+      if (a.top) enter(v, v[0], in, (int)c0);
+    };
     const Vec<T>* xv = reinterpret_cast<const Vec<T>*>(x + c0 + head);
+    if (kw == 0 && head) single(c0, (int)head);
+    first = true;                                          // the few values in front do not make a bar
     for (int64_t i0 = (int64_t)kw * 64; i0 < body; i0 += (int64_t)W * 64) {
       const bool in = i0 + lane < body;
       float v[NV];
@@ -168,27 +214,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
         for (int e = 0; e < NV; ++e) s.add(v[e]);
       } else {
 #pragma unroll
-        for (int e = 0; e < NV; ++e) v[e] = 0.f;
+        for (int e = 0; e < NV; ++e) v[e] = -INFINITY;
       }
-      if (a.top) {
-        uint64_t todo = __ballot(in && (!(vm <= top.bar) || s.l != s.l));
-        while (todo) {                                     // in ascending order of the classes
-          const int o = __ffsll((unsigned long long)todo) - 1;
-#pragma unroll
-          for (int e = 0; e < NV; ++e)
-            top.insert(__builtin_amdgcn_readlane(key_of(v[e]), o), (int)(c0 + head + (i0 + o) * NV) + e, lane, a.top);
-          todo &= todo - 1;
-          todo &= __ballot(in && (!(vm <= top.bar) || s.l != s.l));
-        }
-      }
+      if (a.top) enter(v, vm, in, (int)(c0 + head + i0 * NV));
     }
-    if (kw == 0 && tail < c1) single(tail + lane, tail + lane < c1);
+    first = false;
+    if (kw == 0 && tail < c1) single(tail, (int)(c1 - tail));
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor(s.m, o, 64), l2 = __shfl_xor(s.l, o, 64), t2 = __shfl_xor(s.t, o, 64);
-    s.join(m2, l2, t2);
-  }
+  s.over_wave();
   if (lane == 0) { sums[wave][0] = s.m; sums[wave][1] = s.l; sums[wave][2] = s.t; }
   if (lane < a.top) cand[W == 1 ? wave : 0][W == 1 ? lane : wave * a.top + lane] = make_int2(top.key, top.idx);
   __syncthreads();
@@ -219,42 +252,142 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
   }
 }
 
-// joins the parts of a row: a block a row; the parts' lists are merged 16 at a time through shared memory
+// joins the parts of a row: a block a row; every wave takes every fourth part's list, 64 entries at a time
 template <typename T>
 __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a) {
-  __shared__ int2 cand[17 * 64], next[64];
+  __shared__ float sums[4][3];
+  __shared__ int2 cand[4 * 64];
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, rec = 3 + 2 * a.top;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rec = 3 + 2 * a.top;
   const float* part = a.ws + row * a.segs * rec;
   Sums s;
-  for (int g = 0; g < a.segs; ++g) s.join(part[(int64_t)g * rec], part[(int64_t)g * rec + 1], part[(int64_t)g * rec + 2]);
-  int have = 0;
-  for (int g0 = 0; g0 < a.segs && a.top; g0 += 16) {
-    const int more = (a.segs - g0 < 16 ? a.segs - g0 : 16) * a.top, n = have + more;
-    for (int i = tid; i < more; i += 256) {
-      const int* p = reinterpret_cast<const int*>(part + (int64_t)(g0 + i / a.top) * rec + 3) + 2 * (i % a.top);
-      cand[have + i] = make_int2(p[0], p[1]);
+  for (int g = tid; g < a.segs; g += 256) s.join(part[(int64_t)g * rec], part[(int64_t)g * rec + 1], part[(int64_t)g * rec + 2]);
+  s.over_wave();
+  if (lane == 0) { sums[wave][0] = s.m; sums[wave][1] = s.l; sums[wave][2] = s.t; }
+  TopList top;
+  const int mine = (a.segs - wave + 3) / 4 * a.top;        // entries of the wave's lists
+  for (int i0 = 0; i0 < mine; i0 += 64) {
+    const int i = i0 + lane;
+    int k = NO_KEY, c = INT32_MAX;
+    if (i < mine) {
+      const int* p = reinterpret_cast<const int*>(part + (int64_t)(wave + 4 * (i / a.top)) * rec + 3) + 2 * (i % a.top);
+      k = p[0];
+      c = p[1];
     }
-    __syncthreads();
-    if (g0 + 16 >= a.segs) {
-      have = n;
-      break;
+    uint64_t todo = __ballot(k != NO_KEY && k >= top.last);
+    while (todo) {
+      const int o = __ffsll((unsigned long long)todo) - 1;
+      todo &= todo - 1;
+      top.insert(__builtin_amdgcn_readlane(k, o), __builtin_amdgcn_readlane(c, o), lane, a.top);
     }
-    if (tid < a.top) next[tid] = make_int2(NO_KEY, 0);
-    __syncthreads();
-    for (int i = tid; i < n; i += 256) {
-      const int2 me = cand[i];
-      if (me.x == NO_KEY) continue;
-      int rank = 0;
-      for (int o = 0; o < n; ++o) rank += cand[o].x > me.x || (cand[o].x == me.x && cand[o].y < me.y);
-      if (rank < a.top) next[rank] = me;
-    }
-    __syncthreads();
-    if (tid < a.top) cand[tid] = next[tid];
-    have = a.top;
-    __syncthreads();
   }
-  finish_row<T>(a, row, s, cand, have, tid, 256);
+  if (lane < a.top) cand[wave * a.top + lane] = make_int2(top.key, top.idx);
+  __syncthreads();
+  Sums all;
+  for (int w = 0; w < 4; ++w) all.join(sums[w][0], sums[w][1], sums[w][2]);
+  finish_row<T>(a, row, all, cand, 4 * a.top, tid, 256);
+}
+
+// Rows of at most 256 classes: 32 lanes a row, E values a lane, everything in registers.  The alternatives are taken out one
+// after the other, a maximum over the lanes each.
+template <int CTRL> __device__ inline float dppf(float x) { return __int_as_float(dpp<CTRL>(__float_as_int(x))); }
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+__device__ inline float max32(float x) {                   // over the 32 lanes of a half wave
+  x = fmaxf(x, dppf<0xB1>(x));
+  x = fmaxf(x, dppf<0x4E>(x));
+  x = fmaxf(x, dppf<0x141>(x));
+  x = fmaxf(x, dppf<0x140>(x));
+  const uintx2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float sum32(float x) {
+  x += dppf<0xB1>(x);
+  x += dppf<0x4E>(x);
+  x += dppf<0x141>(x);
+  x += dppf<0x140>(x);
+  const uintx2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ inline void better(int& k, int& i, int k2, int i2) {
+  const bool b = k2 > k || (k2 == k && i2 < i);
+  k = b ? k2 : k;
+  i = b ? i2 : i;
+}
+__device__ inline void best32(int& k, int& i) {
+  better(k, i, dpp<0xB1>(k), dpp<0xB1>(i));
+  better(k, i, dpp<0x4E>(k), dpp<0x4E>(i));
+  better(k, i, dpp<0x141>(k), dpp<0x141>(i));
+  better(k, i, dpp<0x140>(k), dpp<0x140>(i));
+  const uintx2 rk = __builtin_amdgcn_permlane16_swap((uint32_t)k, (uint32_t)k, false, false);
+  const uintx2 ri = __builtin_amdgcn_permlane16_swap((uint32_t)i, (uint32_t)i, false, false);
+  k = (int)rk[0];
+  i = (int)ri[0];
+  better(k, i, (int)rk[1], (int)ri[1]);
+}
+
+template <typename T, int E>
+__global__ __launch_bounds__(256) void score_short_kernel(ScoreArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const bool live = row < a.rows;                          // both halves of a wave go through the same steps
+  const T* x = reinterpret_cast<const T*>(a.logits) + (live ? row : 0) * a.ld;
+  float v[E];
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int c = lane + 32 * e;
+    v[e] = c < a.V ? value_of(x[c]) : -INFINITY;
+    m = fmaxf(m, v[e]);
+  }
+  const int64_t y = a.tokens && live ? a.tokens[row * a.ld_tok] - a.tok_sub : -1;
+  m = max32(m);
+  float l = 0.f, t = 0.f;
+  const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float d = v[e] - ms, w = __builtin_amdgcn_exp2f(d * LOG2E);
+    l += w;
+    t = fmaf(w, fmaxf(d, -1e30f), t);
+  }
+  l = sum32(l);
+  t = sum32(t);
+  const bool none = l == 0.f;
+  const float L = logf(l);
+  const bool token = y >= 0 && y < a.V;
+  float lp = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (lane + 32 * e == (token ? (int)y : -1)) lp = none ? -INFINITY : l != l ? l : v[e] - m - L;
+  if (live && (token ? lane == ((int)y & 31) : lane == 0)) a.logp[row * a.ld_logp] = lp;
+  if (live && lane == 0) {
+    a.entropy[row * a.ld_ent] = none ? 0.f : L - t / l;
+    if (a.stat) {
+      a.stat[2 * row] = m;
+      a.stat[2 * row + 1] = L;
+    }
+  }
+  if (a.top == 0) return;
+  int key[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) key[e] = lane + 32 * e < a.V ? key_of(v[e]) : NO_KEY;
+  for (int n0 = 0; n0 < a.top; n0 += 32) {                 // lane i keeps alternative n0 + i
+    int mk = NO_KEY, mi = 0;
+    const int n1 = a.top - n0 < 32 ? a.top - n0 : 32;
+    for (int n = 0; n < n1; ++n) {
+      int k = NO_KEY, i = INT32_MAX;
+#pragma unroll
+      for (int e = 0; e < E; ++e) better(k, i, key[e], lane + 32 * e);
+      best32(k, i);
+      if (lane == n) { mk = k; mi = i; }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (lane + 32 * e == i) key[e] = NO_KEY;
+    }
+    if (live && lane < n1) {
+      a.top_ids[row * a.top + n0 + lane] = mi;
+      a.top_logp[row * a.top + n0 + lane] = none ? -INFINITY : l != l ? l : of_key(mk) - m - L;
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ gradient
@@ -332,15 +465,67 @@ __global__ __launch_bounds__(256) void score_bwd_kernel(ScoreBwdArgs a) {
   }
 }
 
+// Rows of at most 256 classes: 32 lanes a row; what a class gets of its own is added up in shared memory first.
+template <typename T>
+__global__ __launch_bounds__(256) void score_short_bwd_kernel(ScoreBwdArgs a) {
+  __shared__ float own[8][256];
+  const int lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 8 + slot;
+  const bool live = row < a.rows;
+  for (int c = lane; c < a.V; c += 32) own[slot][c] = 0.f;
+  __syncthreads();
+  float pull = 0.f;
+  if (live && a.g_logp && a.tokens) {
+    const int64_t y = a.tokens[row * a.ld_tok] - a.tok_sub;
+    if (y >= 0 && y < a.V) {
+      pull = a.g_logp[row];
+      if (lane == 0) own[slot][y] = pull;
+    }
+  }
+  __syncthreads();
+  float sum = 0.f;
+  if (live)
+    for (int t = lane; t < a.top; t += 32) {                            // the alternatives are different classes
+      const float g = a.g_top[row * a.top + t];
+      const int64_t id = a.top_ids[row * a.top + t];
+      if (id >= 0 && id < a.V) own[slot][id] += g;
+      sum += g;
+    }
+  pull += sum32(sum);
+  __syncthreads();
+  if (!live) return;
+  const float M = a.stat[2 * row], L = a.stat[2 * row + 1], H = a.entropy[row * a.ld_ent], gh = a.g_entropy ? a.g_entropy[row] : 0.f;
+  const bool none = M == -INFINITY && L == -INFINITY;
+  const T* x = reinterpret_cast<const T*>(a.logits) + row * a.ld;
+  T* dx = reinterpret_cast<T*>(a.dx) + row * a.V;
+  for (int c = lane; c < a.V; c += 32) {
+    const float v = value_of(x[c]), lp = (v - M) - L, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+    const float r = own[slot][c] - p * (pull + gh * (fmaxf(lp, -1e30f) + H));
+    put(dx + c, none || v == -INFINITY ? 0.f : r);
+  }
+}
+
 int type_bytes(int dtype) { return dtype == TVAE_F32 ? 4 : dtype == TVAE_BF16 || dtype == TVAE_F16 ? 2 : 0; }
 
 template <typename T>
 void launch_score(const ScoreArgs& a, hipStream_t s) {
-  if (a.segs == 1 && a.V <= 2048)
-    hipLaunchKernelGGL((score_kernel<T, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((score_kernel<T, 4>), dim3((unsigned)a.rows, a.segs), dim3(256), 0, s, a);
+  if (a.V <= 256) {
+    const dim3 grid((unsigned)((a.rows + 7) / 8)), block(256);
+    if (a.V <= 32) hipLaunchKernelGGL((score_short_kernel<T, 1>), grid, block, 0, s, a);
+    else if (a.V <= 64) hipLaunchKernelGGL((score_short_kernel<T, 2>), grid, block, 0, s, a);
+    else if (a.V <= 128) hipLaunchKernelGGL((score_short_kernel<T, 4>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((score_short_kernel<T, 8>), grid, block, 0, s, a);
+    return;
+  }
+  if (a.segs == 1 && a.V <= 2048) hipLaunchKernelGGL((score_kernel<T, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((score_kernel<T, 4>), dim3((unsigned)a.rows, a.segs), dim3(256), 0, s, a);
   if (a.segs > 1) hipLaunchKernelGGL((score_join_kernel<T>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
+}
+
+template <typename T>
+void launch_bwd(const ScoreBwdArgs& a, hipStream_t s) {
+  if (a.V <= 256) hipLaunchKernelGGL(score_short_bwd_kernel<T>, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(score_bwd_kernel<T>, dim3((unsigned)a.rows, (unsigned)((a.V + a.seg_len - 1) / a.seg_len)), dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -353,7 +538,7 @@ extern "C" int tvae_token_logp(const void* logits, int64_t ld, int dtype, const 
              (long long)V, (long long)ld, top);
   TVAE_CHECK(type_bytes(dtype), TVAE_E_DTYPE, "tvae_token_logp: dtype %d is not TVAE_F32, TVAE_BF16 or TVAE_F16", dtype);
   if (rows == 0) return TVAE_OK;
-  TVAE_CHECK(logits && logp && entropy && stat && (top == 0 || (top_logp && top_ids)), TVAE_E_NULL, "tvae_token_logp: null pointer");
+  TVAE_CHECK(logits && logp && entropy && (top == 0 || (top_logp && top_ids)), TVAE_E_NULL, "tvae_token_logp: null pointer");
   TVAE_CHECK((uintptr_t)logits % type_bytes(dtype) == 0, TVAE_E_SHAPE, "tvae_token_logp: logits are not aligned to their type");
   TVAE_CHECK(segs >= 1 && segs <= 1024 && (segs == 1 || ws), TVAE_E_SHAPE, "tvae_token_logp: 1 .. 1024 parts, more than one with a workspace");
   TVAE_CHECK(rows <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_token_logp: too many rows in one call (%lld)", (long long)rows);
@@ -380,13 +565,12 @@ extern "C" int tvae_token_logp_bwd(const void* logits, int64_t ld, int dtype, co
              "tvae_token_logp_bwd: logits or dx are not aligned to their type");
   TVAE_CHECK(rows <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_token_logp_bwd: too many rows in one call (%lld)", (long long)rows);
   const int64_t seg_len = 16384;
-  const dim3 grid((unsigned)rows, (unsigned)((V + seg_len - 1) / seg_len));
-  TVAE_CHECK(grid.y <= 65535, TVAE_E_SHAPE, "tvae_token_logp_bwd: V too large (%lld)", (long long)V);
+  TVAE_CHECK((V + seg_len - 1) / seg_len <= 65535, TVAE_E_SHAPE, "tvae_token_logp_bwd: V too large (%lld)", (long long)V);
   ScoreBwdArgs a = {logits, dx, tokens, top_ids, stat, entropy, g_logp, g_entropy, g_top, ld, ld_tok, tok_sub, rows, V, ld_ent, seg_len,
                     g_top ? top : 0};
-  if (dtype == TVAE_F32) hipLaunchKernelGGL(score_bwd_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else if (dtype == TVAE_BF16) hipLaunchKernelGGL(score_bwd_kernel<B16>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL(score_bwd_kernel<F16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  if (dtype == TVAE_F32) launch_bwd<float>(a, (hipStream_t)stream);
+  else if (dtype == TVAE_BF16) launch_bwd<B16>(a, (hipStream_t)stream);
+  else launch_bwd<F16>(a, (hipStream_t)stream);
   TVAE_LAUNCH_CHECK("tvae_token_logp_bwd");
   return TVAE_OK;
 }

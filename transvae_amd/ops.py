@@ -1326,7 +1326,7 @@ def token_logp(logits, tokens, top=0, tok_sub=0, out=None):
 
 def score_segments(rows, V):
     "parts that a row of V logits is cut into"
-    return max(1, min(-(-V // 8192), 1024 // max(1, rows)))
+    return max(1, min(-(-V // 2048), 1024 // max(1, rows))) if V > 2048 else 1
 
 
 class TokenLogpFn(torch.autograd.Function):
