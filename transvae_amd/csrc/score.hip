@@ -73,36 +73,37 @@ struct Sums {
 
 template <int CTRL> __device__ inline int dpp(int x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false); }
 
+// the n-th largest of the lanes' keys (n = 1 .. 64): a bitonic sort across the wave, descending
+__device__ inline int nth_key(int k, int lane, int n) {
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1) {
+#pragma unroll
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      const int other = __shfl_xor(k, d, 64);
+      const bool up = (lane & size) != 0, low = (lane & d) == 0;
+      k = (low != up) ? max(k, other) : min(k, other);
+    }
+  }
+  return __builtin_amdgcn_readlane(k, n - 1);
+}
+
 // A wave's best: lane i < top holds the i-th (by descending key, then ascending class).
 struct TopList {
   int key = NO_KEY, idx = INT32_MAX;
-  int last = NO_KEY;                                       // key of entry top - 1, the same in all lanes
-  float bar = __int_as_float(0x7FC00000);                  // its value; NaN while the list is not full: nothing is <= NaN
   __device__ inline void insert(int k, int i, int lane, int top) {      // k, i uniform
     const int pos = __popcll(__ballot(lane < top && (key > k || (key == k && idx < i))));
     if (pos >= top) return;
     const int ku = dpp<0x138>(key), iu = dpp<0x138>(idx);  // one lane up (wave_shr:1)
     if (lane > pos) { key = ku; idx = iu; }
     if (lane == pos) { key = k; idx = i; }
-    last = __builtin_amdgcn_readlane(key, top - 1);
-    bar = last == NO_KEY ? __int_as_float(0x7FC00000) : of_key(last);
   }
-  // A bar before the list has one: the top-th largest of the lanes' own maxima.  That many values reach it, so nothing below
-  // it can be among the best.
-  static __device__ inline float opening_bar(float vm, int lane, int top) {
-    int k = key_of(vm);
-#pragma unroll
-    for (int size = 2; size <= 64; size <<= 1) {           // a bitonic sort across the lanes, descending
-#pragma unroll
-      for (int d = size >> 1; d > 0; d >>= 1) {
-        const int other = __shfl_xor(k, d, 64);
-        const bool up = (lane & size) != 0, low = (lane & d) == 0;
-        k = (low != up) ? max(k, other) : min(k, other);
-      }
-    }
-    return of_key(__builtin_amdgcn_readlane(k, top - 1));
-  }
+  __device__ inline int entry(int n) const { return __builtin_amdgcn_readlane(key, n); }
 };
+// the largest float below every value of key k: v > bar_below(k) is key(v) >= k, NaN included
+__device__ inline float bar_below(int k) {
+  if (k == NO_KEY) return __int_as_float(0x7FC00000);      // nothing is <= NaN
+  return of_key(k == 0 ? -2 : k - 1);                      // -1 is the key that -0 does not have
+}
 
 struct ScoreArgs {
   const void* logits;
@@ -148,6 +149,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
   constexpr int NV = Vec<T>::N;
   __shared__ float sums[W == 1 ? 4 : W][3];
   __shared__ int2 cand[W == 1 ? 4 : W][64];
+  // W > 1: each wave's `share`-th best key so far.  W shares are `top` values, so `top` values of the row reach the least of
+  // them; a stale one is only lower, so the waves do not wait for each other to read them
+  __shared__ volatile int pub[4];
+  const int share = (a.top + W - 1) / W;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   const int kw = W == 1 ? 0 : wave;
@@ -161,20 +166,19 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
     int64_t head = ((16 - ((uintptr_t)(x + c0) & 15)) & 15) / sizeof(T);              // values up to a 16-byte border
     if (head > c1 - c0) head = c1 - c0;
     const int64_t body = (c1 - c0 - head) / NV, tail = c0 + head + body * NV;
-    // enters what of v[0 .. N) (lane o's values are classes base + o * N ..) is above the bar that stood before this step; all
-    // earlier entries are lower classes, so equal values behind them stay out, and equal values of one step are told apart
-    // by their class
-    bool first = true;
+    // Enters what of v[0 .. N) (lane o's values are classes base + o * N ..) can be among the best.  `own`: the last entry of the
+    // wave's list; what equals it is a higher class than all entries and stays out.  `floor`: a key that at least `top` values of
+    // the row reach; what equals it may still count.
+    int own = NO_KEY, floor = NO_KEY;
+    float bar = __int_as_float(0x7FC00000);
+    auto set_bar = [&]() { bar = floor > own ? bar_below(floor) : own == NO_KEY ? __int_as_float(0x7FC00000) : of_key(own); };
     auto enter = [&](auto& v, float vm, bool in, int base) {
       constexpr int N = sizeof(v) / sizeof(float);
-      const bool opening = first;
-      const float bar = opening ? TopList::opening_bar(in ? vm : -INFINITY, lane, a.top) : top.bar;
-      first = false;
       const bool odd = s.l != s.l;                         // a NaN went by: the maximum may have passed over it
-      if (!__any(in && (odd || (opening ? !(vm < bar) : !(vm <= bar))))) return;
+      if (!__any(in && (odd || !(vm <= bar)))) return;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        uint64_t todo = __ballot(in && (opening ? !(v[e] < bar) : !(v[e] <= bar)));
+        uint64_t todo = __ballot(in && !(v[e] <= bar));
         if (!todo) continue;
         const int k = key_of(v[e]);
         while (todo) {
@@ -183,6 +187,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
           top.insert(__builtin_amdgcn_readlane(k, o), base + o * N + e, lane, a.top);
         }
       }
+      own = top.entry(a.top - 1);
+      if (W > 1) {
+        const int q = top.entry(share - 1);
+        if (lane == 0 && q != NO_KEY) pub[wave] = q;
+      }
+      set_bar();
     };
     auto single = [&](int64_t c0, int n) {                 // one value a lane
       const bool in = lane < n;
@@ -195,8 +205,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
     };
     const Vec<T>* xv = reinterpret_cast<const Vec<T>*>(x + c0 + head);
     if (kw == 0 && head) single(c0, (int)head);
-    first = true;                                          // the few values in front do not make a bar
-    for (int64_t i0 = (int64_t)kw * 64; i0 < body; i0 += (int64_t)W * 64) {
+    bool opening = a.top > 0;
+    for (int64_t i0 = (int64_t)kw * 64; i0 < body || opening; i0 += (int64_t)W * 64) {
       const bool in = i0 + lane < body;
       float v[NV];
       float vm = -INFINITY;
@@ -216,9 +226,31 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
 #pragma unroll
         for (int e = 0; e < NV; ++e) v[e] = -INFINITY;
       }
-      if (a.top) enter(v, vm, in, (int)(c0 + head + i0 * NV));
+      if (a.top) {
+        if (opening) {                                     // every wave of the block comes by here once
+          const int q = nth_key(key_of(vm), lane, share);
+          if (W > 1) {
+            if (lane == 0) pub[wave] = q;
+            __syncthreads();
+          } else {
+            floor = q;
+          }
+          opening = false;
+        }
+        if (W > 1) {
+          int f = pub[0];
+#pragma unroll
+          for (int w = 1; w < W; ++w) f = min(f, pub[w]);
+          if (f > floor) {
+            floor = f;
+            set_bar();
+          }
+        } else {
+          set_bar();
+        }
+        enter(v, vm, in, (int)(c0 + head + i0 * NV));
+      }
     }
-    first = false;
     if (kw == 0 && tail < c1) single(tail, (int)(c1 - tail));
   }
   s.over_wave();
@@ -274,7 +306,9 @@ __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a) {
       k = p[0];
       c = p[1];
     }
-    uint64_t todo = __ballot(k != NO_KEY && k >= top.last);
+    // of the first 64 only the best `top` can stay, later on what is not below the last entry
+    const int bar = i0 == 0 ? nth_key(k, lane, a.top) : top.entry(a.top - 1);
+    uint64_t todo = __ballot(k != NO_KEY && k >= bar);
     while (todo) {
       const int o = __ffsll((unsigned long long)todo) - 1;
       todo &= todo - 1;

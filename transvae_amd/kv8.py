@@ -11,18 +11,18 @@ import torch
 
 from . import ops
 from ._lib import BF16, F16, F32, TvaeError, call
-from .ops import _p
+from .ops import _ptr
 
 _TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 DK = (32, 64, 128, 256)
 
 
-def _rows(t, name, n_dims=4):
+def _rows(t, name):
     "t as rows that the kernels take: dense in the last dimension, every row on a 16-byte border (copied only if it is not)"
-    if t.dim() != n_dims or t.dtype not in _TYPES:
-        raise TvaeError("%s must be a %d-dimensional float32, bfloat16 or float16 tensor (got %s %s)" % (name, n_dims, tuple(t.shape), t.dtype))
-    per = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % per for s in t.stride()[:-1]):
+    if t.dim() != 4 or t.dtype not in _TYPES:
+        raise TvaeError("%s must be a 4-dimensional float32, bfloat16 or float16 tensor (got %s %s)" % (name, tuple(t.shape), t.dtype))
+    a, b, c, one = t.stride()
+    if one != 1 or (t.data_ptr() | (a | b | c) * t.element_size()) & 15:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -43,8 +43,9 @@ class KV8Cache:
         if k.dim() != 4 or v.shape != k.shape or k_exp.shape != k.shape[:2] or v_exp.shape != k_exp.shape:
             raise TvaeError("cache: codes must be (n_pages, heads, page, dk) and exponents (n_pages, heads), got %s %s %s %s"
                             % (tuple(k.shape), tuple(v.shape), tuple(k_exp.shape), tuple(v_exp.shape)))
+        dev = k.device
         for t in (k, v, k_exp, v_exp):
-            if t.dtype != torch.uint8 or not t.is_contiguous() or t.device != k.device:
+            if t.dtype is not torch.uint8 or t.device != dev or not t.is_contiguous():
                 raise TvaeError("cache: codes and exponents must be contiguous uint8 tensors of one device")
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.n_pages, self.heads, self.page, self.dk = k.shape
@@ -76,35 +77,34 @@ class KV8Cache:
         return t
 
     def _pages(self, table, n):
-        "(pointer of the block table or None, pages a sequence) for a call over n sequences (None: as many as there are)"
+        "(address of the block table or 0, pages a sequence, sequences) for a call over n sequences (None: as many as there are)"
         if table is None:
             if self.n_seq is None:
                 raise TvaeError("a cache without sequences of its own needs a block table")
             if n is not None and n != self.n_seq:
                 raise TvaeError("%d sequences, but the cache belongs to %d" % (n, self.n_seq))
-            return None, self.n_pages // self.n_seq, self.n_seq
+            return 0, self.n_pages // self.n_seq, self.n_seq
         if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.shape[1] < 1 or (n is not None and table.shape[0] != n):
             raise TvaeError("block table must be a contiguous int32 (sequences, pages) tensor%s, got %s %s"
                             % ("" if n is None else " of %d sequences" % n, table.dtype, tuple(table.shape)))
-        return _p(self._on(table, "block table")), table.shape[1], table.shape[0]
+        return _ptr(self._on(table, "block table")), table.shape[1], table.shape[0]
 
     def _ints(self, x, n, name):
-        "(pointer or None, number): per-sequence int32 values, or one number for all of them"
+        "(address or 0, number): per-sequence int32 values, or one number for all of them"
         if x is None or not torch.is_tensor(x):
-            return None, 0 if x is None else int(x)
+            return 0, 0 if x is None else int(x)
         if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] != n or not x.is_contiguous():
             raise TvaeError("%s must be a number or a contiguous int32 tensor of %d values, got %s %s" % (name, n, x.dtype, tuple(x.shape)))
-        return _p(self._on(x, name)), 0
+        return _ptr(self._on(x, name)), 0
 
     def _cache_args(self):
-        return _p(self.k), _p(self.v), _p(self.k_exp), _p(self.v_exp), self.n_pages
+        return _ptr(self.k), _ptr(self.v), _ptr(self.k_exp), _ptr(self.v_exp), self.n_pages
 
     def _call(self, name, *args):
         "on the cache's device, whichever is current, and on that device's current stream"
         ops.call_on(self.device, name, *args)
 
     # ------------------------------------------------------------------------------------------ operators
-    @torch.no_grad()
     def store(self, k, v, start=0, count=None, table=None):
         """Rows t < count[b] (None: all) of k, v (n, T, heads, dk) become tokens start[b] + t of sequence b.  `start` and
         `count` are numbers or int32 (n,) tensors on the device.  Overwriting from the middle of a sequence leaves what
@@ -120,10 +120,9 @@ class KV8Cache:
             T, count = min(T, max(0, int(count))), None
         sp, s0 = self._ints(start, n, "start")
         cp, _ = self._ints(count, n, "count")
-        self._call("tvae_kv8_store", _p(k), *k.stride()[:3], _p(v), *v.stride()[:3], _TYPES[k.dtype], *self._cache_args(), tab, per,
+        self._call("tvae_kv8_store", _ptr(k), *k.stride()[:3], _ptr(v), *v.stride()[:3], _TYPES[k.dtype], *self._cache_args(), tab, per,
                    sp, s0, cp, n, T, self.heads, self.dk, self.page)
 
-    @torch.no_grad()
     def load(self, T, start=0, count=None, table=None, dtype=torch.float32):
         """(k, v), each (n, T, heads, dk) of `dtype`: tokens start[b] .. start[b] + T - 1 of every sequence, zeros from
         count[b] on and where a sequence has no such token."""
@@ -135,10 +134,9 @@ class KV8Cache:
             count = torch.full((n,), int(count), dtype=torch.int32, device=self.device)
         cp, _ = self._ints(count, n, "count")
         k, v = (torch.empty((n, T, self.heads, self.dk), dtype=dtype, device=self.device) for _ in range(2))
-        self._call("tvae_kv8_load", *self._cache_args(), tab, per, sp, s0, cp, _p(k), _p(v), _TYPES[dtype], n, T, self.heads, self.dk, self.page)
+        self._call("tvae_kv8_load", *self._cache_args(), tab, per, sp, s0, cp, _ptr(k), _ptr(v), _TYPES[dtype], n, T, self.heads, self.dk, self.page)
         return k, v
 
-    @torch.no_grad()
     def attend(self, q, lens, table=None, causal=True, key_mask=None, scale=None, out=None, splits=None):
         """softmax(scale q k^T) v: q (n, Lq, G * heads, dk), query head i over key head i // G, the first lens[b] tokens of
         every sequence (a number or an int32 (n,) tensor).  The Lq queries are the LAST tokens of what lens counts: with
@@ -153,7 +151,7 @@ class KV8Cache:
         self._on(q, "q")
         tab, per, _ = self._pages(table, n)
         lp, l0 = self._ints(lens, n, "lens")
-        mp, ldm, mw = None, 0, 0
+        mp, ldm, mw = 0, 0, 0
         if key_mask is not None:
             if key_mask.dim() != 2 or key_mask.shape[0] != n or key_mask.dtype not in (torch.bool, torch.uint8):
                 raise TvaeError("attend: key_mask must be a bool or uint8 (n, W) tensor, got %s %s" % (key_mask.dtype, tuple(key_mask.shape)))
@@ -161,7 +159,7 @@ class KV8Cache:
             if (mw > 1 and key_mask.stride(1) != 1) or key_mask.stride(0) < mw:       # also an expanded row
                 key_mask = key_mask.contiguous()
             ldm = max(key_mask.stride(0), mw)
-            mp = _p(self._on(key_mask, "key_mask") if mw else self.k_exp)             # no column: nothing is visible, nothing is read
+            mp = _ptr(self._on(key_mask, "key_mask") if mw else self.k_exp)             # no column: nothing is visible, nothing is read
         if out is None:
             o = out = torch.empty((n, Lq, hq, dk), dtype=q.dtype, device=q.device)
         else:
@@ -170,15 +168,16 @@ class KV8Cache:
             self._on(out, "out")
             o = _rows(out, "out")
         if splits is None:
-            splits = self._splits(n, hq // self.heads * Lq, per * self.page if lp is not None else l0)
+            splits = self._splits(n, hq // self.heads * Lq, per * self.page if lp else l0)
         ws = None
         if splits > 1:
             ws = torch.empty(n * Lq * hq * splits * (dk + 2), dtype=torch.float32, device=q.device)
-        self._call("tvae_kv8_attn", _p(q), *q.stride()[:3], _p(o), *o.stride()[:3], _TYPES[q.dtype], *self._cache_args(), tab, per,
+        self._call("tvae_kv8_attn", _ptr(q), *q.stride()[:3], _ptr(o), *o.stride()[:3], _TYPES[q.dtype], *self._cache_args(), tab, per,
                    lp, l0, mp, ldm, mw, int(causal), n, self.heads, hq // self.heads, Lq, dk, self.page,
-                   1.0 / math.sqrt(dk) if scale is None else float(scale), splits, _p(ws))
+                   1.0 / math.sqrt(dk) if scale is None else float(scale), splits, _ptr(ws))
         if o is not out:
-            out.copy_(o)
+            with torch.no_grad():
+                out.copy_(o)
         return out
 
     def _splits(self, n, rows, keys):

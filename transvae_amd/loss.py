@@ -53,6 +53,12 @@ def token_logprobs(logits, tokens=None, top=0):
         if tokens.shape != lead or tokens.is_floating_point() or tokens.dtype == torch.bool or tokens.device != logits.device:
             raise ops._lib.TvaeError("token_logprobs: tokens must be integers of shape %s on %s, got %s %s on %s"
                                      % (tuple(lead), logits.device, tuple(tokens.shape), tokens.dtype, tokens.device))
-        tokens = tokens.reshape(-1).long()
-    logp, entropy, top_logp, top_ids = ops.TokenLogpFn.apply(logits, tokens, int(top))
+        if tokens.dim() != 1 or tokens.dtype != torch.int64:
+            tokens = tokens.reshape(-1).long()
+    if logits.requires_grad and torch.is_grad_enabled():
+        logp, entropy, top_logp, top_ids = ops.TokenLogpFn.apply(logits, tokens, int(top))
+    else:
+        logp, entropy, _, top_logp, top_ids = ops.token_logp(logits, tokens, int(top))
+    if logits.dim() == 2:
+        return logp, entropy, top_logp, top_ids
     return logp.view(lead), entropy.view(lead), top_logp.view(*lead, top), top_ids.view(*lead, top)

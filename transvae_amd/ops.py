@@ -157,7 +157,7 @@ def _stream():
 def call_on(device, name, *args):
     "one entry point on `device` and its current stream, whichever device is current (the stream is the last argument of all of them)"
     if _cur_device is not None and _cur_device() == device.index:
-        return call(name, *args, _stream())
+        return call(name, *args, _raw_stream(device.index))
     with torch.cuda.device(device):
         call(name, *args, _stream())
 
@@ -1306,21 +1306,27 @@ def _logit_rows(logits):
     return lg, lg.stride(0) if lg.shape[0] > 1 else V
 
 
-def token_logp(logits, tokens, top=0, tok_sub=0, out=None):
+def _ptr(t):
+    "device address of a tensor as a plain number, 0 for None: _p without the ctypes object (argtypes take numbers too)"
+    if t is None:
+        return 0
+    return t.data_ptr() if t.is_cuda else _p(t)
+
+
+def token_logp(logits, tokens, top=0, tok_sub=0, out=None, stat=False):
     """Raw launcher behind loss.token_logprobs: logits (rows, V) of row stride ld, tokens (rows,) int64 (any stride) or None, less
-    `tok_sub`.  Returns (logp, entropy, stat, top_logp, top_ids); `out` = (logp, entropy) may be strided (rows,) fp32 buffers."""
+    `tok_sub`.  Returns (logp, entropy, stat or None, top_logp, top_ids); `out` = (logp, entropy) may be strided (rows,) fp32 buffers."""
     lg, ld = _logit_rows(logits)
     rows, V = lg.shape
     dev = lg.device
-    logp, entropy = out if out is not None else (torch.empty(rows, device=dev, dtype=torch.float32) for _ in range(2))
-    stat = torch.empty((rows, 2), device=dev, dtype=torch.float32)
-    top_logp = torch.empty((rows, top), device=dev, dtype=torch.float32)
-    top_ids = torch.empty((rows, top), device=dev, dtype=torch.int64)
+    logp, entropy = out if out is not None else (torch.empty(rows, device=dev, dtype=torch.float32), torch.empty(rows, device=dev, dtype=torch.float32))
+    stat = torch.empty((rows, 2), device=dev, dtype=torch.float32) if stat else None
+    top_logp, top_ids = torch.empty((rows, top), device=dev, dtype=torch.float32), torch.empty((rows, top), device=dev, dtype=torch.int64)
     segs = score_segments(rows, V)
     ws = torch.empty(rows * segs * (3 + 2 * top), device=dev, dtype=torch.float32) if segs > 1 else None
-    call_on(dev, "tvae_token_logp", _p(lg), ld, LOGIT_TYPES[lg.dtype], _p(tokens), 1 if tokens is None else tokens.stride(0), int(tok_sub),
-            rows, V, top, _p(logp), logp.stride(0), _p(entropy), entropy.stride(0), _p(stat), _p(top_logp) if top else None,
-            _p(top_ids) if top else None, segs, _p(ws))
+    call_on(dev, "tvae_token_logp", _ptr(lg), ld, LOGIT_TYPES[lg.dtype], _ptr(tokens), 1 if tokens is None else tokens.stride(0), int(tok_sub),
+            rows, V, top, _ptr(logp), logp.stride(0), _ptr(entropy), entropy.stride(0), _ptr(stat), _ptr(top_logp) if top else 0,
+            _ptr(top_ids) if top else 0, segs, _ptr(ws))
     return logp, entropy, stat, top_logp, top_ids
 
 
@@ -1334,7 +1340,7 @@ class TokenLogpFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, top):
-        logp, entropy, stat, top_logp, top_ids = token_logp(logits, tokens, top)
+        logp, entropy, stat, top_logp, top_ids = token_logp(logits, tokens, top, stat=True)
         ctx.save_for_backward(logits, tokens, stat, entropy, top_ids)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_ids)
@@ -1349,8 +1355,8 @@ class TokenLogpFn(torch.autograd.Function):
         top = top_ids.shape[1]
         dx = torch.empty((rows, V), device=lg.device, dtype=lg.dtype)
         g_logp, g_entropy, g_top = (None if g is None else _c(g.to(torch.float32)) for g in (g_logp, g_entropy, g_top if top else None))
-        call_on(lg.device, "tvae_token_logp_bwd", _p(lg), ld, LOGIT_TYPES[lg.dtype], _p(tokens), 1 if tokens is None else tokens.stride(0), 0,
-                rows, V, top, _p(stat), _p(entropy), 1, _p(top_ids) if top else None, _p(g_logp), _p(g_entropy), _p(g_top), _p(dx))
+        call_on(lg.device, "tvae_token_logp_bwd", _ptr(lg), ld, LOGIT_TYPES[lg.dtype], _ptr(tokens), 1 if tokens is None else tokens.stride(0), 0,
+                rows, V, top, _ptr(stat), _ptr(entropy), 1, _ptr(top_ids) if top else 0, _ptr(g_logp), _ptr(g_entropy), _ptr(g_top), _ptr(dx))
         return dx.view(logits.shape), None, None
 
 
