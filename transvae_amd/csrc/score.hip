@@ -39,6 +39,21 @@ __device__ inline int key_of(float x) {
 }
 __device__ inline float of_key(int k) { return k == INT32_MAX ? __int_as_float(0x7FC00000) : __int_as_float(k < 0 ? k ^ 0x7FFFFFFF : k); }
 
+template <int CTRL> __device__ inline int dpp(int x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false); }
+template <int CTRL> __device__ inline float dppf(float x) { return __int_as_float(dpp<CTRL>(__float_as_int(x))); }
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+// the value of lane ^ D, without shared memory: quad permutes, mirrors of 8 (^ 7) and 16 (^ 15) lanes, row swaps
+template <int D> __device__ inline int lane_xor(int x, int lane) {
+  if (D == 1) return dpp<0xB1>(x);
+  if (D == 2) return dpp<0x4E>(x);
+  if (D == 4) return dpp<0x1B>(dpp<0x141>(x));
+  if (D == 8) return dpp<0x141>(dpp<0x140>(x));
+  const uintx2 r = D == 16 ? __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false)
+                           : __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+  return (int)(lane & D ? r[0] : r[1]);
+}
+template <int D> __device__ inline float lane_xorf(float x, int lane) { return __int_as_float(lane_xor<D>(__float_as_int(x), lane)); }
+
 struct Sums {
   float m = -INFINITY, l = 0.f, t = 0.f;
   __device__ inline void grow(float to) {                  // to > m
@@ -54,12 +69,25 @@ struct Sums {
     l += e;
     t = fmaf(e, fmaxf(d, -1e30f), t);                      // -inf adds 0, not 0 * inf
   }
-  __device__ inline void over_wave() {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), t2 = __shfl_xor(t, o, 64);
-      join(m2, l2, t2);
-    }
+  __device__ inline void over_wave(int lane) {             // every lane ends with the sums of all
+    float M = m;
+    M = fmaxf(M, dppf<0xB1>(M));
+    M = fmaxf(M, dppf<0x4E>(M));
+    M = fmaxf(M, dppf<0x141>(M));
+    M = fmaxf(M, dppf<0x140>(M));
+    M = fmaxf(M, lane_xorf<16>(M, lane));
+    M = fmaxf(M, lane_xorf<32>(M, lane));
+    if (M > m) grow(M);
+    l = total(l, lane);
+    t = total(t, lane);
+  }
+  static __device__ inline float total(float x, int lane) {
+    x += dppf<0xB1>(x);
+    x += dppf<0x4E>(x);
+    x += dppf<0x141>(x);
+    x += dppf<0x140>(x);
+    x += lane_xorf<16>(x, lane);
+    return x + lane_xorf<32>(x, lane);
   }
   __device__ inline void join(float m2, float l2, float t2) {
     if (m2 > m) grow(m2);
@@ -71,19 +99,23 @@ struct Sums {
   }
 };
 
-template <int CTRL> __device__ inline int dpp(int x) { return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false); }
-
 // the n-th largest of the lanes' keys (n = 1 .. 64): a bitonic sort across the wave, descending
+template <int SIZE, int D> __device__ inline void sort_step(int& k, int lane) {
+  const int other = lane_xor<D>(k, lane);
+  const bool up = (lane & SIZE) != 0, low = (lane & D) == 0;
+  k = (low != up) ? max(k, other) : min(k, other);
+}
+template <int SIZE, int D> __device__ inline void sort_steps(int& k, int lane) {
+  sort_step<SIZE, D>(k, lane);
+  if constexpr (D > 1) sort_steps<SIZE, D / 2>(k, lane);
+}
 __device__ inline int nth_key(int k, int lane, int n) {
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1) {
-#pragma unroll
-    for (int d = size >> 1; d > 0; d >>= 1) {
-      const int other = __shfl_xor(k, d, 64);
-      const bool up = (lane & size) != 0, low = (lane & d) == 0;
-      k = (low != up) ? max(k, other) : min(k, other);
-    }
-  }
+  sort_steps<2, 1>(k, lane);
+  sort_steps<4, 2>(k, lane);
+  sort_steps<8, 4>(k, lane);
+  sort_steps<16, 8>(k, lane);
+  sort_steps<32, 16>(k, lane);
+  sort_steps<64, 32>(k, lane);
   return __builtin_amdgcn_readlane(k, n - 1);
 }
 
@@ -146,12 +178,12 @@ __device__ inline void finish_row(const ScoreArgs& a, int64_t row, const Sums& s
 // W waves share a row (or one part of it); W == 1: a block has four rows.
 template <typename T, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs a) {
-  constexpr int NV = Vec<T>::N;
+  constexpr int NV = Vec<T>::N, H = 8 / NV;
   __shared__ float sums[W == 1 ? 4 : W][3];
   __shared__ int2 cand[W == 1 ? 4 : W][64];
   // W > 1: each wave's `share`-th best key so far.  W shares are `top` values, so `top` values of the row reach the least of
   // them; a stale one is only lower, so the waves do not wait for each other to read them
-  __shared__ volatile int pub[4];
+  __shared__ int pub[4];
   const int share = (a.top + W - 1) / W;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
@@ -190,7 +222,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
       own = top.entry(a.top - 1);
       if (W > 1) {
         const int q = top.entry(share - 1);
-        if (lane == 0 && q != NO_KEY) pub[wave] = q;
+        if (lane == 0 && q != NO_KEY) __hip_atomic_store(&pub[wave], q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
       set_bar();
     };
@@ -206,54 +238,73 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
     const Vec<T>* xv = reinterpret_cast<const Vec<T>*>(x + c0 + head);
     if (kw == 0 && head) single(c0, (int)head);
     bool opening = a.top > 0;
-    for (int64_t i0 = (int64_t)kw * 64; i0 < body || opening; i0 += (int64_t)W * 64) {
-      const bool in = i0 + lane < body;
-      float v[NV];
-      float vm = -INFINITY;
-      if (in) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(xv + i0 + lane);
+    // eight values a lane and step, the next eight in flight meanwhile (sixteen cost 16-bit logits their occupancy: 4096 x 32000
+    // bf16 with 4 alternatives 100 us against 91)
+    constexpr int64_t STEP = (int64_t)W * 64;
+    int64_t i0 = (int64_t)kw * 64;
+    uint4 ahead[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      ahead[h] = make_uint4(0, 0, 0, 0);
+      if (i0 + h * STEP + lane < body) ahead[h] = *reinterpret_cast<const uint4*>(xv + i0 + h * STEP + lane);
+    }
+    for (; i0 < body || opening; i0 += H * STEP) {
+      float v[H][NV];
+      float vm[H];
+      bool in[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        vm[h] = -INFINITY;
+        in[h] = i0 + h * STEP + lane < body;
         Vec<T> t;
-        *reinterpret_cast<uint4*>(t.x) = raw;
+        *reinterpret_cast<uint4*>(t.x) = ahead[h];
 #pragma unroll
         for (int e = 0; e < NV; ++e) {
-          v[e] = value_of(t.x[e]);
-          vm = fmaxf(vm, v[e]);
+          v[h][e] = in[h] ? value_of(t.x[e]) : -INFINITY;
+          vm[h] = fmaxf(vm[h], v[h][e]);
         }
-        if (vm > s.m) s.grow(vm);
+      }
 #pragma unroll
-        for (int e = 0; e < NV; ++e) s.add(v[e]);
-      } else {
+      for (int h = 0; h < H; ++h)
+        if (i0 + (H + h) * STEP + lane < body) ahead[h] = *reinterpret_cast<const uint4*>(xv + i0 + (H + h) * STEP + lane);
+      const float both = fmaxf(vm[0], vm[H - 1]);
+      if (both > s.m) s.grow(both);
 #pragma unroll
-        for (int e = 0; e < NV; ++e) v[e] = -INFINITY;
+      for (int h = 0; h < H; ++h) {
+#pragma unroll
+        for (int e = 0; e < NV; ++e) s.add(v[h][e]);       // -inf where there is no value: adds nothing
       }
       if (a.top) {
         if (opening) {                                     // every wave of the block comes by here once
-          const int q = nth_key(key_of(vm), lane, share);
+          const int q = nth_key(key_of(both), lane, share);
           if (W > 1) {
-            if (lane == 0) pub[wave] = q;
+            if (lane == 0) __hip_atomic_store(&pub[wave], q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             __syncthreads();
           } else {
             floor = q;
+            set_bar();
           }
           opening = false;
         }
-        if (W > 1) {
-          int f = pub[0];
+        const bool odd = s.l != s.l;                       // a NaN went by: the maximum may have passed over it
+        if (__any(odd || !(both <= bar))) {
+          if (W > 1) {                                     // how far the others are is only looked up when it matters
+            int f = INT32_MAX;
 #pragma unroll
-          for (int w = 1; w < W; ++w) f = min(f, pub[w]);
-          if (f > floor) {
-            floor = f;
-            set_bar();
+            for (int w = 0; w < W; ++w) f = min(f, __hip_atomic_load(&pub[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+            if (f > floor) {
+              floor = f;
+              set_bar();
+            }
           }
-        } else {
-          set_bar();
+#pragma unroll
+          for (int h = 0; h < H; ++h) enter(v[h], vm[h], in[h], (int)(c0 + head + (i0 + h * STEP) * NV));
         }
-        enter(v, vm, in, (int)(c0 + head + i0 * NV));
       }
     }
     if (kw == 0 && tail < c1) single(tail, (int)(c1 - tail));
   }
-  s.over_wave();
+  s.over_wave(lane);
   if (lane == 0) { sums[wave][0] = s.m; sums[wave][1] = s.l; sums[wave][2] = s.t; }
   if (lane < a.top) cand[W == 1 ? wave : 0][W == 1 ? lane : wave * a.top + lane] = make_int2(top.key, top.idx);
   __syncthreads();
@@ -294,7 +345,7 @@ __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a) {
   const float* part = a.ws + row * a.segs * rec;
   Sums s;
   for (int g = tid; g < a.segs; g += 256) s.join(part[(int64_t)g * rec], part[(int64_t)g * rec + 1], part[(int64_t)g * rec + 2]);
-  s.over_wave();
+  s.over_wave(lane);
   if (lane == 0) { sums[wave][0] = s.m; sums[wave][1] = s.l; sums[wave][2] = s.t; }
   TopList top;
   const int mine = (a.segs - wave + 3) / 4 * a.top;        // entries of the wave's lists
@@ -324,8 +375,6 @@ __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a) {
 
 // Rows of at most 256 classes: 32 lanes a row, E values a lane, everything in registers.  The alternatives are taken out one
 // after the other, a maximum over the lanes each.
-template <int CTRL> __device__ inline float dppf(float x) { return __int_as_float(dpp<CTRL>(__float_as_int(x))); }
-typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 __device__ inline float max32(float x) {                   // over the 32 lanes of a half wave
   x = fmaxf(x, dppf<0xB1>(x));
   x = fmaxf(x, dppf<0x4E>(x));
