@@ -69,6 +69,11 @@ struct Sums {
     l += e;
     t = fmaf(e, fmaxf(d, -1e30f), t);                      // -inf adds 0, not 0 * inf
   }
+  __device__ inline void add_finite(float x) {             // m and x are finite, m at least x; a NaN passes too
+    const float d = x - m, e = __builtin_amdgcn_exp2f(d * LOG2E);
+    l += e;
+    t = fmaf(e, d, t);
+  }
   __device__ inline void over_wave(int lane) {             // every lane ends with the sums of all
     float M = m;
     M = fmaxf(M, dppf<0xB1>(M));
@@ -99,7 +104,7 @@ struct Sums {
   }
 };
 
-// the n-th largest of the lanes' keys (n = 1 .. 64): a bitonic sort across the wave, descending
+// the n-th largest of the lanes' keys (n = 1 .. 64), for many by a bitonic sort across the wave, descending
 template <int SIZE, int D> __device__ inline void sort_step(int& k, int lane) {
   const int other = lane_xor<D>(k, lane);
   const bool up = (lane & SIZE) != 0, low = (lane & D) == 0;
@@ -109,7 +114,22 @@ template <int SIZE, int D> __device__ inline void sort_steps(int& k, int lane) {
   sort_step<SIZE, D>(k, lane);
   if constexpr (D > 1) sort_steps<SIZE, D / 2>(k, lane);
 }
+__device__ inline int max_key(int k, int lane) {
+  k = max(k, dpp<0xB1>(k));
+  k = max(k, dpp<0x4E>(k));
+  k = max(k, dpp<0x141>(k));
+  k = max(k, dpp<0x140>(k));
+  k = max(k, lane_xor<16>(k, lane));
+  return max(k, lane_xor<32>(k, lane));
+}
 __device__ inline int nth_key(int k, int lane, int n) {
+  if (n <= 8) {                                            // n maxima taken out one by one are fewer steps than the sort's 21
+    for (int i = 1; i < n; ++i) {
+      const int m = max_key(k, lane);
+      if (lane == __ffsll((unsigned long long)__ballot(k == m)) - 1) k = NO_KEY;
+    }
+    return max_key(k, lane);
+  }
   sort_steps<2, 1>(k, lane);
   sort_steps<4, 2>(k, lane);
   sort_steps<8, 4>(k, lane);
@@ -250,18 +270,31 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
     }
     for (; i0 < body || opening; i0 += H * STEP) {
       float v[H][NV];
-      float vm[H];
+      float vm[H], least = INFINITY;
       bool in[H];
+      const bool whole = i0 + (H - 1) * STEP + 64 <= body; // every lane has its values: the same for all of them
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         vm[h] = -INFINITY;
-        in[h] = i0 + h * STEP + lane < body;
+        in[h] = whole || i0 + h * STEP + lane < body;
         Vec<T> t;
         *reinterpret_cast<uint4*>(t.x) = ahead[h];
 #pragma unroll
+        for (int e = 0; e < NV; ++e) v[h][e] = value_of(t.x[e]);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+          for (int e = 0; e < NV; ++e) v[h][e] = in[h] ? v[h][e] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+#pragma unroll
         for (int e = 0; e < NV; ++e) {
-          v[h][e] = in[h] ? value_of(t.x[e]) : -INFINITY;
           vm[h] = fmaxf(vm[h], v[h][e]);
+          least = fminf(least, v[h][e]);
         }
       }
 #pragma unroll
@@ -269,10 +302,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
         if (i0 + (H + h) * STEP + lane < body) ahead[h] = *reinterpret_cast<const uint4*>(xv + i0 + (H + h) * STEP + lane);
       const float both = fmaxf(vm[0], vm[H - 1]);
       if (both > s.m) s.grow(both);
+      if (__all(least > -INFINITY && s.m < INFINITY && s.m > -INFINITY)) {    // masked classes want more care: -inf adds 0, not 0 * inf
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
+        for (int h = 0; h < H; ++h) {
 #pragma unroll
-        for (int e = 0; e < NV; ++e) s.add(v[h][e]);       // -inf where there is no value: adds nothing
+          for (int e = 0; e < NV; ++e) s.add_finite(v[h][e]);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+#pragma unroll
+          for (int e = 0; e < NV; ++e) s.add(v[h][e]);
+        }
       }
       if (a.top) {
         if (opening) {                                     // every wave of the block comes by here once
