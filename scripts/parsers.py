@@ -58,6 +58,9 @@ def sample_parser():
         ('--k', _opt(15, int)), ('--condition', _opt('', str)), ('--entropy_cutoff', _opt(5, float)),
         ('--n_samples', _opt(30000, int)), ('--n_samples_per_batch', _opt(100, int)),
         ('--save_path', _opt(None, str)),
+        # additions (no counterpart in the reference)
+        ('--kv_cache', dict(default='fp32', choices=['fp32', 'fp8'], type=str)),   # fp8: 8-bit caches (transvae only)
+        ('--scores', _SWITCH),                                                     # a second column: each molecule's log likelihood
     ])
 
 

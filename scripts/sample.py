@@ -9,7 +9,7 @@ import pandas as pd
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from scripts.parsers import model_load, sample_parser  # noqa: E402
-from transvae_amd.tvae_util import calc_entropy, decode_mols  # noqa: E402
+from transvae_amd.tvae_util import calc_entropy, decode_mols, sequence_logp  # noqa: E402
 
 
 def sample(args):
@@ -41,25 +41,40 @@ def sample(args):
         return -(-share // args.n_samples_per_batch)
     import torch
     dev = vae._device()
+    logp = torch.empty(0, device=dev) if args.scores else None
+    ids = torch.empty((0, vae.tgt_len), dtype=torch.uint8, device=dev)            # on the model's device even when empty
     if os.environ.get('TVAE_SAMPLE_PER_BATCH') == '1':
-        ids = [vae.sample(args.n_samples_per_batch, sample_mode=sample_mode, sample_dims=sample_dims, k=args.k,
-                          condition=condition, return_str=False).to(torch.uint8) for _ in range(n_batches(rank))]
-        ids = torch.cat(ids) if ids else torch.empty((0, vae.tgt_len), dtype=torch.uint8, device=dev)
+        got = [vae.sample(args.n_samples_per_batch, sample_mode=sample_mode, sample_dims=sample_dims, k=args.k,
+                          condition=condition, return_str=False, kv_cache=args.kv_cache, scores=args.scores)
+               for _ in range(n_batches(rank))]
+        if got and args.scores:
+            logp = torch.cat([g[1] for g in got])
+            got = [g[0] for g in got]
+        if got:
+            ids = torch.cat([g.to(torch.uint8) for g in got])
     else:
         zs = [vae.sample_from_memory(args.n_samples_per_batch, mode=sample_mode, sample_dims=sample_dims, k=args.k)
               for _ in range(n_batches(rank))]
-        ids = vae.decode_latents(torch.cat(zs), condition=condition) if zs \
-            else torch.empty((0, vae.tgt_len), dtype=torch.uint8, device=dev)     # on the model's device even when empty
+        if zs:
+            ids = vae.decode_latents(torch.cat(zs), condition=condition, kv_cache=args.kv_cache, scores=args.scores)
+            if args.scores:
+                ids, logp, _ = ids
+                logp = sequence_logp(ids, logp, vae.params['CHAR_DICT']['<end>'])
     if world > 1:
         rows = [n_batches(r) * args.n_samples_per_batch for r in range(world)]
-        padded = torch.zeros((max(rows), ids.shape[1]), dtype=torch.uint8, device=ids.device)
-        padded[:ids.shape[0]] = ids
-        if dist.get_backend() == 'gloo':
-            padded = padded.cpu()
-        parts = [torch.empty_like(padded) for _ in range(world)] if rank == 0 else None
-        dist.gather(padded, parts, dst=0)
-        if rank == 0:
-            ids = torch.cat([part[:n] for part, n in zip(parts, rows)])
+
+        def gathered(x):
+            "rank 0: the rows of all ranks; the others: their own"
+            padded = torch.zeros((max(rows),) + x.shape[1:], dtype=x.dtype, device=x.device)
+            padded[:x.shape[0]] = x
+            if dist.get_backend() == 'gloo':
+                padded = padded.cpu()
+            parts = [torch.empty_like(padded) for _ in range(world)] if rank == 0 else None
+            dist.gather(padded, parts, dst=0)
+            return torch.cat([part[:n] for part, n in zip(parts, rows)]) if rank == 0 else x
+        ids = gathered(ids)
+        if args.scores:
+            logp = gathered(logp)
         dist.destroy_process_group()
     samples = decode_mols(ids, vae.params['ORG_DICT']) if rank == 0 else []
     if rank == 0:
@@ -67,7 +82,10 @@ def sample(args):
         if save_path is None:
             os.makedirs('generated', exist_ok=True)
             save_path = 'generated/{}_{}.csv'.format(vae.name, args.sample_mode)
-        pd.DataFrame(samples, columns=['mol']).to_csv(save_path, index=False)
+        table = pd.DataFrame(samples, columns=['mol'])
+        if args.scores:
+            table['logp'] = logp.cpu().numpy()
+        table.to_csv(save_path, index=False)
 
 
 if __name__ == '__main__':

@@ -141,3 +141,16 @@ def test_python_side_refuses():
               lambda: token_logprobs(torch.zeros(2, 100), top=65), lambda: token_logprobs(torch.tensor(1.0)), lambda: token_logprobs(x)):
         with pytest.raises(E):
             c()
+
+
+def test_sequence_logp_stops_behind_the_first_end():
+    from transvae_amd.tvae_util import sequence_logp
+    ids = torch.tensor([[3, 25, 7, 25], [1, 2, 3, 4], [25, 25, 25, 25]], dtype=torch.uint8)
+    logp = torch.tensor([[-1.0, -2.0, -4.0, -8.0]] * 3)
+    assert sequence_logp(ids, logp, 25).tolist() == [-3.0, -15.0, -1.0]
+
+
+def test_decoder_refuses_an_unknown_cache():
+    from transvae_amd.decode import GreedyDecoder
+    with pytest.raises(_lib().TvaeError):
+        GreedyDecoder(None, 4, kv_cache="int8")

@@ -485,9 +485,9 @@ import numpy as np  # noqa: E402
 
 from .data import DeviceDataset, DeviceLoader, make_src_mask, make_std_mask, vae_data_gen  # noqa: E402
 from .decode import GreedyDecoder, GRAPH_MAX_N  # noqa: E402
-from .loss import trans_vae_loss, vae_loss  # noqa: E402, F401
+from .loss import token_logprobs, trans_vae_loss, vae_loss  # noqa: E402, F401
 from .opt import Adam, NoamOpt  # noqa: E402
-from .tvae_util import KLAnnealer, decode_mols  # noqa: E402
+from .tvae_util import KLAnnealer, decode_mols, sequence_logp  # noqa: E402
 
 _DEFAULTS = (('BATCH_SIZE', 500), ('BATCH_CHUNKS', 5), ('BETA_INIT', 1e-8), ('BETA', 0.05),
              ('ANNEAL_START', 0), ('WARMUP_STEPS', 10000), ('EPS_SCALE', 1))
@@ -812,14 +812,18 @@ class VAEShell():
             z[:, d] = torch.randn(size)
         return z
 
-    def greedy_decode(self, mem, src_mask=None, condition=[]):
+    def greedy_decode(self, mem, src_mask=None, condition=[], kv_cache='fp32', scores=False):
         """Greedy token ids (n, 125) from latent vectors (reference :383-436), computed by the
-        KV-cached decoder.  `src_mask` (n,1,127), when given, replaces the predicted-length mask."""
+        KV-cached decoder.  `src_mask` (n,1,127), when given, replaces the predicted-length mask.
+        Additions: kv_cache='fp8' keeps the caches in 8 bits (a quarter of the bytes; tokens may differ where two logits are
+        close; transformer only); scores=True returns (ids, logp, entropy) with the log probability of every token, the
+        given ones included, and the entropy of its position, (n, 125) fp32 each."""
         dev = self._device()
         mem = mem.to(dev).float()
         n = mem.shape[0]
         if self.model_type != 'transformer':
-            return self._rnn_greedy_decode(mem, condition)
+            self._fp32_cache_only(kv_cache)
+            return self._rnn_greedy_decode(mem, condition, scores)
         if src_mask is None:
             lens = self.model.encoder.predict_mask_length(mem)            # (n, 1) int64, may be 0
             key_mask = (torch.arange(self.src_len + 1, device=dev)[None, :] < lens).to(torch.uint8).contiguous()
@@ -831,15 +835,20 @@ class VAEShell():
         was_training = self.model.training
         self.model.eval()
         try:
-            return GreedyDecoder(self.model, self.params['h']).run(
+            return GreedyDecoder(self.model, self.params['h'], kv_cache, scores).run(
                 mem, key_mask, self.params['CHAR_DICT']['<start>'], cond, self.tgt_len)
         finally:
             self.model.train(was_training)
 
     DECODE_SLAB = 65536     # latents in flight in decode_latents: ~110 GB of K/V caches for trans4x-256
 
+    @staticmethod
+    def _fp32_cache_only(kv_cache):
+        if kv_cache != 'fp32':
+            raise ops._lib.TvaeError("kv_cache=%r: a recurrent model keeps no key/value cache" % (kv_cache,))
+
     @torch.no_grad()
-    def decode_latents(self, mem, condition=[], slab=None):
+    def decode_latents(self, mem, condition=[], slab=None, kv_cache='fp32', scores=False):
         """greedy_decode over ANY number of latents, `slab` rows (default DECODE_SLAB) in flight at a time; the token ids come
         back as ONE (n, 125) uint8 tensor on the device (the vocabulary has 26 entries: 1 M molecules are 125 MB instead of
         1 GB of int64).  Rows are independent and the kernels sum in a fixed order, so the tokens equal those of
@@ -848,17 +857,24 @@ class VAEShell():
         streams (GreedyDecoder.run_iter): one piece's attention over its K/V caches is HBM-bound, another's projections
         are MFMA-bound, and they overlap -- measured on 262,144 latents: 35.9 / 36.0 k molecules/s on one stream,
         36.5-37.4 k with two pieces, 37.3-37.8 k with three, 38.0 / 38.1 k with four (tools/debug/ab_decode.sh).
-        TVAE_DECODE_STREAMS=1..4 sets the number; 1 decodes whole slabs one after the other on the current stream."""
+        TVAE_DECODE_STREAMS=1..4 sets the number; 1 decodes whole slabs one after the other on the current stream.
+          kv_cache, scores: as in greedy_decode; with scores (ids, logp, entropy) come back."""
         slab = int(slab or os.environ.get("TVAE_DECODE_SLAB") or self.DECODE_SLAB)
         dev = self._device()
         n = mem.shape[0]
-        out = torch.empty((n, self.tgt_len), dtype=torch.uint8, device=dev)
+        out = [torch.empty((n, self.tgt_len), dtype=torch.uint8, device=dev)]
+        if scores:
+            out += [torch.empty((n, self.tgt_len), dtype=torch.float32, device=dev) for _ in range(2)]
+
+        def keep(a, b, got):
+            for whole, part in zip(out, got if scores else (got,)):
+                whole[a:b] = part.to(whole.dtype)
         ways = max(1, min(4, int(os.environ.get("TVAE_DECODE_STREAMS", "4"))))
         half = (slab + ways - 1) // ways
         if self.model_type != 'transformer' or dev.type != 'cuda' or half <= GRAPH_MAX_N or n <= half or ways == 1:
             for s0 in range(0, n, slab):
-                out[s0:s0 + slab] = self.greedy_decode(mem[s0:s0 + slab], condition=condition).to(torch.uint8)
-            return out
+                keep(s0, s0 + slab, self.greedy_decode(mem[s0:s0 + slab], condition=condition, kv_cache=kv_cache, scores=scores))
+            return tuple(out) if scores else out[0]
         mem = mem.to(dev).float()
         cond = [self.params['CHAR_DICT'][tok] for tok in condition]
         start = self.params['CHAR_DICT']['<start>']
@@ -867,7 +883,7 @@ class VAEShell():
         was_training = self.model.training
         self.model.eval()
         try:
-            decoder = GreedyDecoder(self.model, self.params['h'])
+            decoder = GreedyDecoder(self.model, self.params['h'], kv_cache, scores)
             for p0 in range(0, n, ways * half):
                 pieces = [(a, min(a + half, n)) for a in range(p0, p0 + ways * half, half) if a < n]
                 for st in streams[1:]:
@@ -883,20 +899,30 @@ class VAEShell():
                 while live:
                     for k in list(live):
                         with torch.cuda.stream(streams[k]):
-                            ids = next(gens[k], None)
-                            if ids is not None:              # the generator's last value
-                                a, b = pieces[k]
-                                out[a:b] = ids.to(torch.uint8)
+                            got = next(gens[k], None)
+                            if got is not None:              # the generator's last value
+                                keep(*pieces[k], got)
                                 live.remove(k)
                                 gens[k] = None               # releases the slab's caches (to that stream's pool)
                 for st in streams[1:]:
                     main.wait_stream(st)
         finally:
             self.model.train(was_training)
-        return out
+        return tuple(out) if scores else out[0]
+
+    def token_scores(self, data, top=0, eps=None):
+        """Log probability of every token of molecules under teacher forcing: `data` is a batch as train_step takes it ((B, 128):
+        start id, tokens, property).  Returns loss.token_logprobs' (logp, entropy, top_logp, top_ids) over (B, 126); padding
+        has logp 0, so logp.sum(1) is a molecule's log likelihood given its latent.  Differentiable: fine-tuning on
+        likelihoods, rewards or entropies is token_scores(...) -> any scalar -> backward().  `eps`: the latent's noise, as in
+        train_step.  No counterpart in the reference."""
+        src, tgt, _, src_mask, tgt_mask = self._chunk_inputs(data.to(self._device(), non_blocking=True))
+        logits = self._model_forward(src, tgt, src_mask, tgt_mask, eps)[0]
+        y = src[:, 1:]
+        return token_logprobs(logits, torch.where(y == self.pad_idx, -1, y - 1), top=top)
 
     @torch.no_grad()
-    def _rnn_greedy_decode(self, mem, condition=[]):
+    def _rnn_greedy_decode(self, mem, condition=[], scores=False):
         """Greedy decoding of the RNN models.  The reference re-runs the whole decoder over the 126-token buffer for every
         new token and reads position i (:425-431); a GRU is causal, so the same tokens come from ONE pass that carries
         the hidden states from step to step: per step the embedded previous token and memory row i go through one GRU
@@ -914,17 +940,21 @@ class VAEShell():
                 tgt[:, j + 1] = self.params['CHAR_DICT'][tok]
             h = [torch.zeros((n, dec.size), device=dev) for _ in range(dec.n_layers)]
             nxt = torch.empty(n, dtype=torch.int32, device=dev)
+            logp, ent = (torch.empty((n, max_len), device=dev) for _ in range(2)) if scores else (None, None)
             for i in range(max_len):
                 x = rows[:, i, :]
                 if dec.teacher_force:
                     x = torch.cat((model.src_embed(tgt[:, i:i + 1])[:, 0, :], x), dim=1)
                 h = dec.gru.step(x.contiguous(), h)
-                if i >= len(condition):
+                if i >= len(condition) or scores:
                     logits = model.generator(dec.norm(h[-1]))
+                if i >= len(condition):
                     ops.call("tvae_argmax_rows", ops._p(logits), logits.stride(0), logits.shape[1], ops._p(nxt), n,
                              ops._stream())
                     tgt[:, i + 1] = nxt.long() + 1
-            return tgt[:, 1:]
+                if scores:
+                    ops.token_logp(logits, tgt[:, i + 1], tok_sub=1, out=(logp[:, i], ent[:, i]))
+            return (tgt[:, 1:], logp, ent) if scores else tgt[:, 1:]
         finally:
             model.train(was_training)
 
@@ -964,10 +994,15 @@ class VAEShell():
         return (decoded_smiles, mems.numpy()) if return_mems else decoded_smiles
 
     def sample(self, n, method='greedy', sample_mode='rand', sample_dims=None, k=None, return_str=True,
-               condition=[]):
-        "sample z, decode greedily, optionally translate to SMILES strings (reference :511-545)"
+               condition=[], kv_cache='fp32', scores=False):
+        """sample z, decode greedily, optionally translate to SMILES strings (reference :511-545).  Additions: kv_cache as in
+        greedy_decode; scores=True returns (molecules, their log likelihoods (n,) given the sampled latents)"""
         mem = self.sample_from_memory(n, mode=sample_mode, sample_dims=sample_dims, k=k)
-        decoded = self.greedy_decode(mem, condition=condition) if method == 'greedy' else None
+        decoded = self.greedy_decode(mem, condition=condition, kv_cache=kv_cache, scores=scores) if method == 'greedy' else None
+        if scores and decoded is not None:
+            decoded, logp, _ = decoded
+            total = sequence_logp(decoded, logp, self.params['CHAR_DICT']['<end>'])
+            return (decode_mols(decoded, self.params['ORG_DICT']) if return_str else decoded), total
         return decode_mols(decoded, self.params['ORG_DICT']) if return_str else decoded
 
     @torch.no_grad()

@@ -109,3 +109,10 @@ def calc_entropy(sample):
     from scipy.stats import entropy
     return np.array([entropy(np.histogram(sample[:, i], bins=1000, range=(-5., 5.), density=True)[0])
                      for i in range(sample.shape[1])])
+
+
+def sequence_logp(ids, logp, end_id):
+    "log likelihood (n,) of decoded molecules: the tokens' logp (n, L) summed up to the first `end_id` of ids (n, L), it included"
+    end = ids == end_id
+    behind = torch.cumsum(end.to(torch.int32), 1) - end.to(torch.int32) > 0
+    return logp.masked_fill(behind, 0.0).sum(1)
