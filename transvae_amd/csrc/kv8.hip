@@ -10,6 +10,7 @@
 #include "common.h"
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 
 namespace {
@@ -473,22 +474,67 @@ __device__ inline int seq_len(const AttnArgs& a, int b) {
   return (int)(len > 0 ? len : 0);
 }
 
+// the value of lane ^ D for D = 2, 4, 8 (within 16 lanes) and, through row swaps, 16 and 32
+template <int D> __device__ inline float lane_xor(float x, int lane) {
+  if (D == 1) return dpp<0xB1>(x);
+  if (D == 2) return dpp<0x4E>(x);
+  if (D == 4) return dpp<0x1B>(dpp<0x141>(x));
+  if (D == 8) return dpp<0x128>(x);
+  const uintx2 r = D == 16 ? __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false)
+                           : __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(lane & D ? r[0] : r[1]);
+}
+// maximum / sum over the lanes that differ in the bits from log2(FROM) up, the same in all of them
+template <int FROM> __device__ inline float across_max(float x, int lane) {
+  if (FROM <= 2) x = fmaxf(x, lane_xor<2>(x, lane));
+  if (FROM <= 4) x = fmaxf(x, lane_xor<4>(x, lane));
+  if (FROM <= 8) x = fmaxf(x, lane_xor<8>(x, lane));
+  x = fmaxf(x, lane_xor<16>(x, lane));
+  return fmaxf(x, lane_xor<32>(x, lane));
+}
+template <int FROM> __device__ inline float across_sum(float x, int lane) {
+  if (FROM <= 2) x += lane_xor<2>(x, lane);
+  if (FROM <= 4) x += lane_xor<4>(x, lane);
+  if (FROM <= 8) x += lane_xor<8>(x, lane);
+  x += lane_xor<16>(x, lane);
+  return x + lane_xor<32>(x, lane);
+}
+// 2 N values a lane -> N: a row swap hands the lower lanes the other half's first N, the upper ones the last N
+template <int D, int N> __device__ inline void fold_rows(float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uintx2 r = D == 32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(x[i]), __float_as_uint(x[i + N]), false, false)
+                             : __builtin_amdgcn_permlane16_swap(__float_as_uint(x[i]), __float_as_uint(x[i + N]), false, false);
+    x[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+}
+template <int D, int N> __device__ inline void fold_lanes(float (&x)[16], int lane) {
+  const bool up = (lane & D) != 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float keep = up ? x[i + N] : x[i], send = up ? x[i] : x[i + N];
+    x[i] = keep + lane_xor<D>(send, lane);
+  }
+}
+
 // One query row at a time, without matrix instructions: DK / 16 lanes share a key (16 codes each), 64 / (DK / 16) keys an
 // instruction, four such groups of keys in flight.  Every lane group keeps a softmax of its own (running maximum, sum, its 16
-// dimensions); they meet once at the end.  Masked keys are not read.
+// dimensions); they meet once at the end, by halving what a lane holds.  A group of keys lies in one page (two at DK = 32 and
+// 16 tokens a page), so its address is wave-uniform; keys that are not visible read the group's first row with the others.
 template <typename T, int DK, int KW>
 __global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
-  constexpr int LPK = DK / 16, NK = 64 / LPK, U = 4, KPI = NK * U;
-  __shared__ float sm[4][DK + 2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = KW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  constexpr int LPK = DK / 16, NK = 64 / LPK, U = 4, KPI = NK * U, NV = DK >= 64 ? DK / 64 : 1;
+  __shared__ float sm[KW == 1 ? 1 : 4][64 * NV + 2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t row = KW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   const int kw = KW == 1 ? 0 : wave;
   if (row >= a.rows) return;                                            // KW == 4: one row per block, uniform
-  const int g = (int)(row % a.G);
-  int64_t rest = row / a.G;
-  const int i = (int)(rest % a.Lq);
-  rest /= a.Lq;
-  const int head = (int)(rest % a.h), b = (int)(rest / a.h);
+  const int64_t this_row = row;
+  const int g = (int)((uint32_t)row % (uint32_t)a.G);
+  row = (uint32_t)row / (uint32_t)a.G;
+  const int i = (int)((uint32_t)row % (uint32_t)a.Lq);
+  row = (uint32_t)row / (uint32_t)a.Lq;
+  const int head = (int)((uint32_t)row % (uint32_t)a.h), b = (int)((uint32_t)row / (uint32_t)a.h);
   const int part = lane % LPK, kg = lane / LPK;
   int end = seq_len(a, b) - (a.causal ? a.Lq - 1 - i : 0);
   const int split = blockIdx.y;
@@ -508,38 +554,58 @@ __global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
   for (int d = 0; d < 16; ++d) o[d] = 0.f;
   const PageRow pages(a.pages, b, a.codes[0]);
   const int shift = 31 - __clz(a.page), pm = a.page - 1;
-  const uint8_t* mk = a.mask ? a.mask + (int64_t)b * a.ld_mask : a.exps[0];
+  const uint8_t* mk = a.mask + (int64_t)b * a.ld_mask;
+  const int row_off = (kg & (NK > 16 ? 15 : NK - 1)) * DK + 16 * part;
   for (int64_t j0 = beg + (int64_t)kw * KPI; j0 < end; j0 += (int64_t)KW * KPI) {
-    // every load goes out without a branch; a key that is not visible reads page 0 instead, which all such keys share
     uint4 kc[U], vc[U];
-    int raw[U], ek[U], ev[U], slot[U];
-    uint8_t mb[U];
-    float s[U];
+    int raw[U][2], ek[U], ev[U];
     bool vis[U];
+    bool none = true;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t j = j0 + u * NK + kg;
-      vis[u] = j < end;
-      const int jj = vis[u] ? (int)j : 0;
-      slot[u] = jj >> shift;
-      raw[u] = pages.ask(slot[u]);
-      mb[u] = mk[a.mask ? (jj < a.mask_w ? jj : 0) : 0];
-      if (a.mask) vis[u] = vis[u] && jj < a.mask_w;
+      const int64_t t = j0 + u * NK;
+      raw[u][0] = pages.ask(t < end ? (int)(t >> shift) : 0);
+      if (NK > 16) raw[u][1] = pages.ask(t + 16 < end ? (int)((t + 16) >> shift) : 0);
+      vis[u] = kg < end - t;
+    }
+    if (a.mask) {
+      uint8_t mb[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = j0 + u * NK + kg;
+        vis[u] = vis[u] && j < a.mask_w;
+        mb[u] = mk[vis[u] ? j : 0];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) vis[u] = vis[u] && mb[u] != 0;
     }
 #pragma unroll
+    for (int u = 0; u < U; ++u) none = none && !vis[u];
+    if (__all(none)) continue;
+#pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int id = pages.page(raw[u], slot[u], vis[u] && (!a.mask || mb[u] != 0));
-      vis[u] = id >= 0;
-      const size_t ph = vis[u] ? (size_t)id * a.h + head : 0;
-      const size_t off = vis[u] ? (ph * a.page + ((int)(j0 + u * NK + kg) & pm)) * DK + 16 * part : 16 * part;
-      kc[u] = *reinterpret_cast<const uint4*>(a.codes[0] + off);
-      vc[u] = *reinterpret_cast<const uint4*>(a.codes[1] + off);
+      const int64_t t = j0 + u * NK;
+      const int id0 = pages.page(raw[u][0], (int)(t >> shift), t < end);
+      int id = id0;
+      if (NK > 16) {
+        const int id1 = pages.page(raw[u][1], (int)((t + 16) >> shift), t + 16 < end);
+        id = kg >= 16 ? id1 : id0;
+      }
+      vis[u] = vis[u] && id >= 0;
+      const size_t ph = (size_t)(id < 0 ? 0 : id) * a.h + head;
+      const size_t at = ph * a.page * DK + (NK > 16 ? ((int)t + (kg & 16)) & pm : (int)t & pm) * DK;
+      const int off = vis[u] ? row_off : 16 * part;
+      kc[u] = *reinterpret_cast<const uint4*>(a.codes[0] + at + off);
+      vc[u] = *reinterpret_cast<const uint4*>(a.codes[1] + at + off);
       ek[u] = a.exps[0][ph];
       ev[u] = a.exps[1][ph];
     }
-    float mn = m;
+    float s[U];
+    float mn = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      s[u] = -INFINITY;
+      if (!__any(vis[u])) continue;
       const uint32_t w[4] = {kc[u].x, kc[u].y, kc[u].z, kc[u].w};
       float acc = 0.f;
 #pragma unroll
@@ -553,14 +619,18 @@ __global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
       s[u] = vis[u] ? acc : -INFINITY;
       mn = fmaxf(mn, s[u]);
     }
-    const float ms = mn == -INFINITY ? 0.f : mn;                        // nothing seen so far: every weight is 0
-    const float al = __builtin_amdgcn_exp2f(m - ms);
-    m = mn;
-    l *= al;
+    if (__any(mn > m + 8.f)) {                                          // weights may exceed 1 by 2^8 before the maximum is raised
+      mn = fmaxf(mn, m);
+      const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= al;
 #pragma unroll
-    for (int d = 0; d < 16; ++d) o[d] *= al;
+      for (int d = 0; d < 16; ++d) o[d] *= al;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;                          // nothing seen so far: every weight is 0
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (!__any(vis[u])) continue;
       const float p = __builtin_amdgcn_exp2f(s[u] - ms);
       l += p;
       const float pv = vis[u] ? p * exp_scale(ev[u]) : 0.f;
@@ -574,64 +644,58 @@ __global__ __launch_bounds__(256) void kv8_attn_row_kernel(AttnArgs a) {
       }
     }
   }
-  // the lane groups meet
-  float M = m;
-#pragma unroll
-  for (int d = LPK; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  // the lane groups meet: 16 dimensions a lane become NV
+  float M = across_max<LPK>(m, lane);
   const float f = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
-  l *= f;
+  l = across_sum<LPK>(l * f, lane);
 #pragma unroll
   for (int d = 0; d < 16; ++d) o[d] *= f;
-#pragma unroll
-  for (int d = LPK; d < 64; d <<= 1) {
-    l += __shfl_xor(l, d, 64);
-#pragma unroll
-    for (int c = 0; c < 16; ++c) o[c] += __shfl_xor(o[c], d, 64);
-  }
+  fold_rows<32, 8>(o);
+  fold_rows<16, 4>(o);
+  if (LPK <= 8) fold_lanes<8, 2>(o, lane);
+  if (LPK <= 4) fold_lanes<4, 1>(o, lane);
+  if (LPK <= 2) o[0] += lane_xor<2>(o[0], lane);
+  const int d0 = 16 * part + (lane >> 5) * 8 + (lane >> 4 & 1) * 4 + (LPK <= 8 ? (lane >> 3 & 1) * 2 : 0) + (LPK <= 4 ? lane >> 2 & 1 : 0);
   if (KW > 1) {
-    if (kg == 0) {
 #pragma unroll
-      for (int c = 0; c < 16; ++c) sm[wave][16 * part + c] = o[c];
-      if (part == 0) { sm[wave][DK] = M; sm[wave][DK + 1] = l; }
-    }
+    for (int c = 0; c < NV; ++c) sm[wave][c * 64 + lane] = o[c];
+    if (lane == 0) { sm[wave][64 * NV] = M; sm[wave][64 * NV + 1] = l; }
     __syncthreads();
     if (wave != 0) return;
-    float MM = -INFINITY;
-    for (int w = 0; w < KW; ++w) MM = fmaxf(MM, sm[w][DK]);
-    const float z = MM == -INFINITY ? 0.f : MM;
+    M = fmaxf(fmaxf(sm[0][64 * NV], sm[1][64 * NV]), fmaxf(sm[2][64 * NV], sm[3][64 * NV]));
+    const float z = M == -INFINITY ? 0.f : M;
     l = 0.f;
 #pragma unroll
-    for (int c = 0; c < 16; ++c) o[c] = 0.f;
+    for (int c = 0; c < NV; ++c) o[c] = 0.f;
+#pragma unroll
     for (int w = 0; w < KW; ++w) {
-      const float r = __builtin_amdgcn_exp2f(sm[w][DK] - z);
-      l += r * sm[w][DK + 1];
+      const float r = __builtin_amdgcn_exp2f(sm[w][64 * NV] - z);
+      l += r * sm[w][64 * NV + 1];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) o[c] += r * sm[w][16 * part + c];
+      for (int c = 0; c < NV; ++c) o[c] += r * sm[w][c * 64 + lane];
     }
-    M = MM;
   }
-  if (kg != 0) return;
+  if (LPK == 2 && (lane & 2)) return;                                   // two lanes hold the same dimension
   if (a.splits > 1) {
-    float* dst = a.ws + (row * a.splits + split) * DK + 16 * part;
+    float* dst = a.ws + (this_row * a.splits + split) * DK + d0;
 #pragma unroll
-    for (int c = 0; c < 16; ++c) dst[c] = o[c];
-    if (part == 0) {
-      float* ml = a.ws + a.rows * a.splits * DK + (row * a.splits + split) * 2;
+    for (int c = 0; c < NV; ++c) dst[c] = o[c];
+    if (lane == 0) {
+      float* ml = a.ws + a.rows * a.splits * DK + (this_row * a.splits + split) * 2;
       ml[0] = M;
       ml[1] = l;
     }
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;                           // no visible key: zeros
-  T* dst = reinterpret_cast<T*>(a.o) + (int64_t)b * a.ldob + (int64_t)i * a.ldoi + (int64_t)(head * a.G + g) * a.ldoh + 16 * part;
+  T* dst = reinterpret_cast<T*>(a.o) + (int64_t)b * a.ldob + (int64_t)i * a.ldoi + (int64_t)(head * a.G + g) * a.ldoh + d0;
 #pragma unroll
-  for (int c = 0; c < 16; ++c) Elem<T>::put(dst + c, o[c] * inv);
+  for (int c = 0; c < NV; ++c) Elem<T>::put(dst + c, o[c] * inv);
 }
 
 // ---- several query rows at once, on the matrix cores
 typedef __bf16 bfx2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bfx8 __attribute__((ext_vector_type(8)));
-typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 
 union Frag {                 // eight bf16 of one lane: an operand of v_mfma_f32_16x16x32_bf16
   uint32_t u[4];
