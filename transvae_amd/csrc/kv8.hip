@@ -875,21 +875,24 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
     // scores: sc[t][i] is the lane's query c of tile t against token t0 + 8 quad + i
     floatx4 sc[NT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) sc[t][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < KS; ++s) {                                      // 2 NT sums side by side: each waits for its own last step only
+      Frag kf[2];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        Frag kf;
-        kf.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s], 1.f, false);
-        kf.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s], 1.f, true);
-        kf.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s + 1], 1.f, false);
-        kf.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s + 1], 1.f, true);
+      for (int i = 0; i < 2; ++i) {
+        kf[i].h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s], 1.f, false);
+        kf[i].h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s], 1.f, true);
+        kf[i].h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s + 1], 1.f, false);
+        kf[i].h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(cur.k[i][2 * s + 1], 1.f, true);
+      }
+#pragma unroll
+      for (int p = NQ - 1; p >= 0; --p) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
-          for (int p = NQ - 1; p >= 0; --p)
-            sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf.v, qf[t][s][p].v, sc[t][i], 0, 0, 0);
+          for (int i = 0; i < 2; ++i)
+            sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i].v, qf[t][s][p].v, sc[t][i], 0, 0, 0);
         }
       }
     }
@@ -1052,6 +1055,33 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
   }
 }
 
+// joins few parts of many rows: a thread per four dimensions of a row
+template <typename T>
+__global__ __launch_bounds__(256) void kv8_attn_join_few_kernel(AttnArgs a, int dk) {
+  const int per = dk >> 2;
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x, r = at / per, d = at - r * per;
+  if (r >= a.rows) return;
+  const uint32_t g = r % a.G, rest = r / a.G, i = rest % a.Lq, bh = rest / a.Lq, head = bh % a.h, b = bh / a.h;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + a.rows * a.splits * dk) + (size_t)r * a.splits;
+  const float4* part = reinterpret_cast<const float4*>(a.ws + (size_t)r * a.splits * dk) + d;
+  float M = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[s].x);
+  const float z = M == -INFINITY ? 0.f : M;
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 o = ml[s];
+    const float f = __builtin_amdgcn_exp2f(o.x - z);
+    const float4 v = part[(size_t)s * per];
+    l = fmaf(f, o.y, l);
+    acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;                           // no visible key: zeros
+  T* dst = reinterpret_cast<T*>(a.o) + (int64_t)b * a.ldob + (int64_t)i * a.ldoi + (int64_t)(head * a.G + g) * a.ldoh + 4 * d;
+  const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  Elem<T>::store4(dst, y);
+}
+
 // joins the parts of a split row: a block a row; DK / 4 threads hold four dimensions each, the others take every so-manieth part
 template <typename T>
 __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a, int dk) {
@@ -1179,7 +1209,8 @@ void launch_attn(const AttnArgs& a, int dk, hipStream_t s) {
   else if (dk == 64) launch_dk<T, 64>(a, s);
   else if (dk == 128) launch_dk<T, 128>(a, s);
   else launch_dk<T, 256>(a, s);
-  if (a.splits > 1) hipLaunchKernelGGL((kv8_attn_join_kernel<T>), dim3((unsigned)a.rows), dim3(256), 0, s, a, dk);
+  if (a.splits > 16) hipLaunchKernelGGL((kv8_attn_join_kernel<T>), dim3((unsigned)a.rows), dim3(256), 0, s, a, dk);
+  else if (a.splits > 1) hipLaunchKernelGGL((kv8_attn_join_few_kernel<T>), dim3((unsigned)((a.rows * (dk / 4) + 255) / 256)), dim3(256), 0, s, a, dk);
 }
 
 }  // namespace
