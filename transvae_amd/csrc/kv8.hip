@@ -748,51 +748,54 @@ __device__ inline float quad_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The codes of 32 tokens as one lane (c = lane & 15, quad = lane >> 4) loads them: for the scores the token rows 8 (c >> 2) +
-// 4 t + (c & 3), t = 0, 1, 16 codes of every 64; for the second product W = DK / 16 codes of each of the tokens 8 quad .. + 7.
+// The codes of 32 tokens as one lane (c = lane & 15, quad = lane >> 4) loads them.  For the scores: token rows c and 16 + c, 16
+// codes of every 64.  For the second product: W = DK / 16 codes of the tokens 4 quad .. + 3 and 16 + 4 quad .. + 3, which are
+// those whose scores the lane will hold.  The two halves of 16 tokens lie in one page each, so both addresses are wave-uniform
+// plus an offset that never changes, and the exponents are wave-uniform too.
 template <int DK>
 struct CodeTile {
   static constexpr int W = DK / 16, KN = W >= 4 ? W : 2, VW = W >= 4 ? DK / 64 : 1;     // dwords of a lane's token row, and of W codes
   uint32_t k[2][KN];
   uint32_t v[8][VW];
-  int ek, ev;                // exponents of the lane's tokens 8 quad .. + 7
+  int ek[2], ev[2];
 
-  // id0, id1: pages of the group's first and last 16 tokens (one page unless pages hold 16)
-  __device__ inline void load(const AttnArgs& a, int head, int id0, int id1, int in_page, int c, int quad) {
+  // id0, id1: pages of the two halves
+  __device__ inline void load(const AttnArgs& a, int head, int id0, int id1, int64_t t0, uint32_t koff, uint32_t voff) {
     const int pm = a.page - 1;
-    const size_t p0 = (size_t)id0 * a.h + head, p1 = (size_t)id1 * a.h + head;
-    const size_t pk = c >= 8 ? p1 : p0, pv = quad >= 2 ? p1 : p0;
-    const uint8_t* p = a.codes[0] + pk * a.page * DK + (in_page + (8 * (c >> 2) & pm) + (c & 3)) * DK;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint8_t* r = p + 4 * i * DK;
+      const size_t ph = (size_t)(i ? id1 : id0) * a.h + head;
+      const size_t at = (ph * a.page + ((int)(t0 + 16 * i) & pm)) * DK;
+      const uint8_t* p = a.codes[0] + at + koff;
       if (DK == 32) {
-        *reinterpret_cast<uint2*>(k[i]) = *reinterpret_cast<const uint2*>(r + 8 * quad);
+        *reinterpret_cast<uint2*>(k[i]) = *reinterpret_cast<const uint2*>(p);
       } else {
 #pragma unroll
-        for (int w = 0; w < DK / 64; ++w) *reinterpret_cast<uint4*>(k[i] + 4 * w) = *reinterpret_cast<const uint4*>(r + 64 * w + 16 * quad);
+        for (int w = 0; w < DK / 64; ++w) *reinterpret_cast<uint4*>(k[i] + 4 * w) = *reinterpret_cast<const uint4*>(p + 64 * w);
       }
-    }
-    ek = a.exps[0][pv];
-    p = a.codes[1] + pv * a.page * DK + (in_page + (8 * quad & pm)) * DK + W * c;
+      p = a.codes[1] + at + voff;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (W == 2) v[j][0] = *reinterpret_cast<const uint16_t*>(p + j * DK);
-      else if (W == 4) v[j][0] = *reinterpret_cast<const uint32_t*>(p + j * DK);
-      else if (W == 8) *reinterpret_cast<uint2*>(v[j]) = *reinterpret_cast<const uint2*>(p + j * DK);
-      else *reinterpret_cast<uint4*>(v[j]) = *reinterpret_cast<const uint4*>(p + j * DK);
+      for (int j = 0; j < 4; ++j) {
+        uint32_t* d = v[4 * i + j];
+        if (W == 2) d[0] = *reinterpret_cast<const uint16_t*>(p + j * DK);
+        else if (W == 4) d[0] = *reinterpret_cast<const uint32_t*>(p + j * DK);
+        else if (W == 8) *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(p + j * DK);
+        else *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(p + j * DK);
+      }
+      ek[i] = a.exps[0][ph];
+      ev[i] = a.exps[1][ph];
     }
-    ev = a.exps[1][pv];
   }
 };
+__device__ inline int token_of(int i, int quad) { return (i >> 2) * 16 + 4 * quad + (i & 3); }      // of a lane's i-th score, within the 32
 
-// Eight tokens' W codes as operands of the second product: group g is dimension W c + g of tokens 8 quad .. + 7, in bf16, scaled.
+// Eight tokens' W codes as operands of the second product: group g is dimension W c + g of the lane's tokens, in bf16, scaled.
 template <int DK>
-__device__ inline void value_frag(Frag& f, const uint32_t (&v)[8][CodeTile<DK>::VW], int w, int g, float scale) {
+__device__ inline void value_frag(Frag& f, const uint32_t (&v)[8][CodeTile<DK>::VW], int w, int g, const float (&scale)[2]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {                                         // bytes {x0, y0, x1, y1} or {x2, y2, x3, y3} of two tokens
     const uint32_t two = __builtin_amdgcn_perm(v[2 * i + 1][w], v[2 * i][w], g < 2 ? 0x05010400u : 0x07030602u);
-    f.h[i] = g & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, scale, false);
+    f.h[i] = g & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, scale[i >> 1], true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, scale[i >> 1], false);
   }
 }
 
@@ -803,19 +806,31 @@ __device__ inline void value_frag(Frag& f, const uint32_t (&v)[8][CodeTile<DK>::
 // score passes it by 2^8: until then weights just exceed 1, which costs no precision and saves the rescaling.
 // KW = 4: the block's waves take every fourth group of 32 tokens and meet at the end; KW = 1: every wave has rows of its own.
 template <typename T, int DK, int NT, int KW>
-__global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv8_attn_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv8_attn_tile_kernel(AttnArgs a) {
   constexpr int W = DK / 16, KS = DK / 32, NQ = Pieces<T>::Q, NP = Pieces<T>::P, VW = CodeTile<DK>::VW, VG = W < 4 ? W : 4;
   constexpr int REGS = NT * (4 * W + 2);
   __shared__ float buf[KW == 1 ? 1 : 2 * REGS * 64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, quad = lane >> 4;
   const int M = a.G * a.Lq, mt = (M + 16 * NT - 1) / (16 * NT);
-  int64_t unit = KW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-  if (unit >= (int64_t)a.n * a.h * mt) return;                          // KW == 4: one unit a block, uniform
-  const int kw = KW == 1 ? 0 : wave, split = blockIdx.y;
-  const int64_t bh_m = unit;
-  const int r0 = (int)(bh_m % mt) * 16 * NT;
-  unit /= mt;
-  const int head = (int)(unit % a.h), b = (int)(unit / a.h);
+  const int kw = KW == 1 ? 0 : wave;
+  // KW == 4: the tiles of one (sequence, key head, part) read the same codes, so they go to one die: blocks are dealt to the eight
+  // dies in turn, each with a cache of its own (12 sequences of 4000 tokens, 7 tiles each: PIECE_BEFORE us with the tiles side by
+  // side, PIECE_AFTER us one behind the other on a die)
+  const uint32_t groups = (uint32_t)a.n * a.h * a.splits;
+  uint32_t group, tile;
+  if (KW == 1) {
+    const uint32_t unit = blockIdx.x * 4 + wave;
+    group = unit / mt;
+    tile = unit - group * mt;
+  } else {
+    const uint32_t at = blockIdx.x >> 3;
+    group = at / mt * 8 + (blockIdx.x & 7);
+    tile = at % mt;
+  }
+  if (group >= groups) return;                                          // KW == 4: one group a block, uniform
+  const int split = (int)(group % a.splits);
+  group /= a.splits;
+  const int head = (int)(group % a.h), b = (int)(group / a.h), r0 = (int)tile * 16 * NT;
   const int len = seq_len(a, b);
   const int64_t beg = (int64_t)split * a.chunk;
   auto end_of = [&](int r) {                                            // tokens that row r sees, in this part
@@ -824,6 +839,8 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
   };
   const int rl = r0 + 16 * NT - 1 < M ? r0 + 16 * NT - 1 : M - 1;
   const int most = end_of(rl), least = end_of(r0);
+  // the sign of the scale goes into the queries: the largest raw score then is the largest score
+  const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f, scale = a.scale == 0.f ? 1.f : fabsf(a.scale);
   Frag qf[NT][KS][NQ];
   int end[NT];
 #pragma unroll
@@ -838,10 +855,10 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
       float x[8], y[4];
       Elem<T>::load4(q + d, y);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = y[i];
+      for (int i = 0; i < 4; ++i) x[i] = y[i] * sign;
       Elem<T>::load4(q + d + 4, y);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 + i] = y[i];
+      for (int i = 0; i < 4; ++i) x[4 + i] = y[i] * sign;
       cut_pieces<NQ>(x, qf[t][s]);
     }
   }
@@ -860,19 +877,20 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
   int64_t t0 = beg + 32 * kw;
   auto ask = [&](int64_t tok) { return pages.ask(tok < most ? (int)(tok >> shift) : 0); };
   auto page = [&](int raw, int64_t tok) { return pages.page(raw, (int)(tok >> shift), tok < most); };
+  const uint32_t koff = c * DK + (DK == 32 ? 8 : 16) * quad, voff = 4 * quad * DK + W * c;
+  bool strange = false;
   // page ids (the same for all lanes) are looked up two groups ahead, codes loaded one group ahead; where there is no page, page 0
   // is read instead
-  CodeTile<DK> cur, nxt;
+  CodeTile<DK> tile0, tile1;
   int ra = ask(t0), rb = ask(t0 + 16);
-  int id0 = page(ra, t0), id1 = page(rb, t0 + 16), nd0, nd1;
+  int id0 = page(ra, t0), id1 = page(rb, t0 + 16);
   ra = ask(t0 + step), rb = ask(t0 + step + 16);
-  cur.load(a, head, id0 < 0 ? 0 : id0, id1 < 0 ? 0 : id1, (int)t0 & pm, c, quad);
-  bool strange = false;
-  for (; t0 < most; t0 += step) {
-    nd0 = page(ra, t0 + step), nd1 = page(rb, t0 + step + 16);
+  tile0.load(a, head, id0 < 0 ? 0 : id0, id1 < 0 ? 0 : id1, t0, koff, voff);
+  auto group_of_32 = [&](CodeTile<DK>& cur, CodeTile<DK>& nxt) {
+    const int nd0 = page(ra, t0 + step), nd1 = page(rb, t0 + step + 16);
     ra = ask(t0 + 2 * step), rb = ask(t0 + 2 * step + 16);
-    nxt.load(a, head, nd0 < 0 ? 0 : nd0, nd1 < 0 ? 0 : nd1, (int)(t0 + step) & pm, c, quad);
-    // scores: sc[t][i] is the lane's query c of tile t against token t0 + 8 quad + i
+    nxt.load(a, head, nd0 < 0 ? 0 : nd0, nd1 < 0 ? 0 : nd1, t0 + step, koff, voff);
+    // raw scores: sc[t][i][e] is the lane's query c of tile t against token t0 + 16 i + 4 quad + e
     floatx4 sc[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -896,28 +914,29 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
         }
       }
     }
+    const float ks[2] = {exp_scale(cur.ek[0]) * scale, exp_scale(cur.ek[1]) * scale};
+    float vs[2] = {exp_scale(cur.ev[0]), exp_scale(cur.ev[1])};
     const bool plain = t0 + 32 <= least && !a.mask && id0 >= 0 && id1 >= 0;      // every row of the unit sees all 32 tokens
-    uint32_t seen = 0xFF;                                               // bit i: token 8 quad + i exists and is not masked
     if (!plain) {
-      if ((quad >= 2 ? id1 : id0) < 0) seen = 0;
+      uint32_t seen = (id0 >= 0 ? 0x0Fu : 0u) | (id1 >= 0 ? 0xF0u : 0u);         // bit i: the lane's i-th token exists and is not masked
       if (a.mask) {
         const uint8_t* mk = a.mask + (int64_t)b * a.ld_mask;
         uint8_t mb[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int64_t j = t0 + 8 * quad + i;
+          const int64_t j = t0 + token_of(i, quad);
           mb[i] = mk[j < a.mask_w ? j : 0];
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (t0 + 8 * quad + i >= a.mask_w || mb[i] == 0) seen &= ~(1u << i);
+          if (t0 + token_of(i, quad) >= a.mask_w || mb[i] == 0) seen &= ~(1u << i);
       }
       // codes that no row sees must not be NaN (0 * NaN is not 0); nor may those that only some rows see: they are taken out
-      // here and put back behind the loop
+      // here and put back behind the loop.  Half a page that nobody sees may hold any exponent.
       const bool some = least < most && t0 + 32 > least;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const bool dead = !(t0 + 8 * quad + i < most) || !(seen >> i & 1);
+        const bool dead = !(t0 + token_of(i, quad) < most) || !(seen >> i & 1);
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           uint32_t x = dead ? 0u : cur.v[i][w];
@@ -929,20 +948,25 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
           cur.v[i][w] = x;
         }
       }
+      if (!(seen & 0x0Fu)) vs[0] = 1.f;
+      if (!(seen & 0xF0u)) vs[1] = 1.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int64_t left = end[t] - t0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!(token_of(i, quad) < left) || !(seen >> i & 1)) sc[t][i >> 2][i & 3] = -INFINITY;
+      }
     }
-    const float ksc = exp_scale(cur.ek) * a.scale, vsc = seen ? exp_scale(cur.ev) : 1.f;   // a page of masked tokens may hold any exponent
     Frag pf[NT][NP];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      float x[8];
+      float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3] * ksc;
-      if (!plain) {
-        const int64_t left = end[t] - (t0 + 8 * quad);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (i < left && (seen >> i & 1)) ? x[i] : -INFINITY;
+      for (int i = 0; i < 2; ++i) {
+        const float top = fmaxf(fmaxf(sc[t][i][0], sc[t][i][1]), fmaxf(sc[t][i][2], sc[t][i][3]));
+        mx = fmaxf(mx, top == -INFINITY ? top : top * ks[i]);           // the exponent of half a page that nobody sees does not count
       }
-      float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
       if (__any(mx > m[t] + 8.f)) {
         mx = fmaxf(m[t], quad_max(mx));
         const float al = __builtin_amdgcn_exp2f(m[t] - (mx == -INFINITY ? 0.f : mx));
@@ -952,9 +976,16 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
         for (int g = 0; g < W; ++g) o[t][g] *= al;
       }
       const float ms = m[t] == -INFINITY ? 0.f : m[t];
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = fmaf(sc[t][i >> 2][i & 3], ks[i >> 2], -ms);
+      if (!plain) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = sc[t][i >> 2][i & 3] == -INFINITY ? -INFINITY : x[i];
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - ms);
+        x[i] = __builtin_amdgcn_exp2f(x[i]);
         l[t] += x[i];
       }
       cut_pieces<NP>(x, pf[t]);
@@ -964,7 +995,7 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
 #pragma unroll
       for (int g = 0; g < VG; ++g) {
         Frag vf;
-        value_frag<DK>(vf, cur.v, w, g, vsc);
+        value_frag<DK>(vf, cur.v, w, g, vs);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -974,7 +1005,12 @@ __global__ __launch_bounds__(256, DK == 256 && Pieces<T>::Q > 1 ? 1 : 2) void kv
       }
     }
     id0 = nd0, id1 = nd1;
-    cur = nxt;
+    t0 += step;
+  };
+  while (t0 < most) {
+    group_of_32(tile0, tile1);
+    if (t0 >= most) break;
+    group_of_32(tile1, tile0);
   }
   if (__any(strange)) {                                                 // NaN for the rows that see it: token by token, rare
     for (int64_t g0 = beg + 32 * kw; g0 < most; g0 += step) {
@@ -1187,16 +1223,16 @@ void launch_row(const AttnArgs& a, hipStream_t s) {
 }
 template <typename T, int DK, int NT>
 void launch_tile(const AttnArgs& a, hipStream_t s) {
-  const int64_t units = (int64_t)a.n * a.h * ((a.G * a.Lq + 16 * NT - 1) / (16 * NT));
-  if (units * a.splits >= 8192)
-    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 1>), dim3((unsigned)((units + 3) / 4), a.splits), dim3(256), 0, s, a);
+  const int64_t tiles = (a.G * a.Lq + 16 * NT - 1) / (16 * NT), groups = (int64_t)a.n * a.h * a.splits, units = groups * tiles;
+  if (units >= 8192)
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 4>), dim3((unsigned)units, a.splits), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 4>), dim3((unsigned)((groups + 7) / 8 * 8 * tiles)), dim3(256), 0, s, a);
 }
 template <typename T, int DK>
 void launch_dk(const AttnArgs& a, hipStream_t s) {
   // tiles of 16 rows a wave: as many as its registers take (queries, sums, scores: DK / 32 * pieces * 4 + DK / 4 + 8 a tile)
-  constexpr int PER = DK / 32 * Pieces<T>::Q * 4 + DK / 4 + 8, MOST = 4 * PER <= 150 ? 4 : 2 * PER <= 150 ? 2 : 1;
+  constexpr int PER = DK / 32 * Pieces<T>::Q * 4 + DK / 4 + 8, MOST = 4 * PER <= 120 ? 4 : 2 * PER <= 120 ? 2 : 1;
   const int M = a.G * a.Lq;
   if (M == 1) launch_row<T, DK>(a, s);
   else if (M <= 16 || MOST == 1) launch_tile<T, DK, 1>(a, s);
