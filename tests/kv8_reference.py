@@ -126,7 +126,7 @@ class Cache:
                     qi, ki, vi = q[b, i, g].double(), kk[see, g // G], vv[see, g // G]
                     w = torch.softmax(ki @ qi * scale, 0)
                     o[b, i, g], wv[b, i, g] = w @ vi, w @ vi.abs()
-                    qk[b, i, g] = (ki.abs() @ qi.abs()).max() * scale
+                    qk[b, i, g] = (ki.abs() @ qi.abs()).max() * abs(scale)
         return o, wv, qk
 
 

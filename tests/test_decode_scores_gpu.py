@@ -198,7 +198,17 @@ def test_recurrent_models_score_and_refuse_the_cache():
         with pytest.raises(_lib.TvaeError):
             call(z, kv_cache="fp8")
     with pytest.raises(_lib.TvaeError):
+        vae.kv_cache_error(z)
+    with pytest.raises(_lib.TvaeError):
         _vae().greedy_decode(_z(3), kv_cache="int4")
+
+
+def test_cache_error_is_that_of_the_codes():
+    "relative error of rounding to e4m3: between a quarter of the half step 2^-4 and the half step, for values well inside the scale's range"
+    vae = _vae("trans4x-256")
+    e = vae.kv_cache_error(_z(40))
+    assert e.shape == (len(vae.model.decoder.layers), 2) and bool((e > 2.0 ** -6).all()) and bool((e < 2.0 ** -4).all())
+    assert torch.equal(e, vae.kv_cache_error(_z(40)))
 
 
 @pytest.mark.parametrize("per_batch", ["0", "1"])

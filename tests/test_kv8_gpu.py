@@ -279,6 +279,21 @@ def test_values_of_a_visible_nan_reach_their_own_row_only():
         assert bool(bad[0, 0, G:2 * G, 7].all()) and int(bad.sum()) == G
 
 
+@pytest.mark.parametrize("Lq,G", [(1, 1), (1, 3), (20, 2)])
+def test_scales_of_either_sign_and_out_of_place_or_in_place(Lq, G):
+    n, h, dk, page, per = 2, 2, 64, 16, 5
+    gpu, ref, _, _ = pair(n, per, h, dk, page, False)
+    fill(gpu, ref)
+    q = torch.randn((n, Lq, h * G, dk), generator=torch.Generator().manual_seed(1)) * 0.2
+    for scale in (-0.125, 0.0, -2.0, 1e-3):
+        want = ref.attend(q, [70, 33], None, per, scale=scale)
+        o = gpu.attend(q.cuda(), ints([70, 33]), scale=scale)
+        lim = attend_bound(want[0], want[1], want[2].abs(), dk, 80, torch.float32)
+        assert bool(((o.cpu().double() - want[0]).abs() <= lim).all()), scale
+        qq = q.cuda()
+        assert torch.equal(gpu.attend(qq, ints([70, 33]), scale=scale, out=qq), o) and torch.equal(qq, o)
+
+
 def test_no_sequences_no_queries_no_keys():
     from transvae_amd.kv8 import KV8Cache
     c = KV8Cache.empty(4, 2, 64, 32, "cuda:0")

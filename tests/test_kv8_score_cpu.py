@@ -70,7 +70,7 @@ def test_load_refuses(bad):
 
 @pytest.mark.parametrize("bad", CACHE + [dict(q=None), dict(o=None), dict(q=ODD), dict(oh=2), dict(G=0), dict(Lq=-1), dict(len0=-1), dict(len0=129),
                                          dict(mask=P, mw=10, ldm=5), dict(mask=P, mw=-1), dict(splits=0), dict(splits=2), dict(splits=2000, ws=P),
-                                         dict(n=1 << 20, table=P, Lq=1 << 12)])
+                                         dict(n=1 << 20, table=P, Lq=1 << 12), dict(splits=4, ws=ODD), dict(n=1 << 19, table=P, Lq=4, splits=1000, ws=P)])
 def test_attend_refuses(bad):
     assert _attn(**bad) < 0 and _lib().lib().tvae_last_error()
 
@@ -130,7 +130,8 @@ def test_python_side_refuses():
              lambda: ok.store(r[:1], r[:1]), lambda: ok.attend(r[:1], 1), lambda: ok.attend(torch.zeros(2, 1, 3, 64), 1), lambda: ok.attend(r, i32(3)),
              lambda: ok.attend(r, torch.zeros(2)), lambda: ok.attend(r, 1, key_mask=torch.zeros(2, 5)), lambda: ok.attend(r, 1, key_mask=torch.zeros(3, 5, dtype=torch.bool)),
              lambda: ok.attend(r, 1, table=i32(3, 2)), lambda: ok.attend(r, 1, table=i32(2, 0)), lambda: ok.attend(r, 1, table=torch.zeros(2, 2)),
-             lambda: ok.attend(r, 1, out=r.half()), lambda: ok.load(3, dtype=torch.float64), lambda: ok.store(r, r, count=torch.zeros(2)),
+             lambda: ok.attend(r, 1, out=r.half()), lambda: ok.attend(r, 1 << 32), lambda: ok.store(r, r, start=1 << 33), lambda: ok.load(1, start=-(1 << 40)),
+             lambda: ok.attend(r, 1, out=torch.zeros(1, 1, 2, 64).expand(2, 1, 2, 64)), lambda: ok.load(3, dtype=torch.float64), lambda: ok.store(r, r, count=torch.zeros(2)),
              lambda: KV8Cache(mk(6, 2, 32, 64), mk(6, 2, 32, 64), mk(6, 2), mk(6, 2)).load(3)]
     for c in calls:
         with pytest.raises(E):

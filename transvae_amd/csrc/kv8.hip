@@ -238,7 +238,8 @@ template <typename T> __device__ inline void put_codes(uint8_t* dst, const Raw<T
 
 // A few rows a sequence (T <= 4: a decode step, drafted tokens).  The lanes that one row's 16-byte pieces take hold the K and
 // the V rows of one (sequence, head) in registers: their maxima, the page's exponents, the codes.  Bound by latency more than
-// by the rows' bytes, hence both sides in one thread.
+// by the rows' bytes, hence both sides in one thread (16384 x 4 heads x 64 fp32, one row: a wave per (sequence, head, side) 69 us,
+// these lane groups with a side each 16 us, with both 12 us = 3.4 TB/s).
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void kv8_append_kernel(StoreArgs a) {
   constexpr int N = Raw<T>::N, LPR = DK / N;
@@ -813,9 +814,9 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv8_attn_tile_kernel(A
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, quad = lane >> 4;
   const int M = a.G * a.Lq, mt = (M + 16 * NT - 1) / (16 * NT);
   const int kw = KW == 1 ? 0 : wave;
-  // KW == 4: the tiles of one (sequence, key head, part) read the same codes, so they go to one die: blocks are dealt to the eight
-  // dies in turn, each with a cache of its own (12 sequences of 4000 tokens, 7 tiles each: PIECE_BEFORE us with the tiles side by
-  // side, PIECE_AFTER us one behind the other on a die)
+  // KW == 4: the tiles of one (sequence, key head, part) read the same codes, so they go to one die, one behind the other: blocks
+  // are dealt to the eight dies in turn, and each has a cache of its own (12 sequences of 4000 tokens, 4 key heads, 7 tiles each,
+  // 3 parts: 68 us with the tiles on different dies, 61 us so)
   const uint32_t groups = (uint32_t)a.n * a.h * a.splits;
   uint32_t group, tile;
   if (KW == 1) {
@@ -1231,7 +1232,9 @@ void launch_tile(const AttnArgs& a, hipStream_t s) {
 }
 template <typename T, int DK>
 void launch_dk(const AttnArgs& a, hipStream_t s) {
-  // tiles of 16 rows a wave: as many as its registers take (queries, sums, scores: DK / 32 * pieces * 4 + DK / 4 + 8 a tile)
+  // tiles of 16 rows a wave: what is unpacked once serves all of them, but two waves a SIMD have to stay (one query sequence of 512
+  // tokens, 32 heads, 8 key heads x 128 bf16, 4000 keys: 1 tile 99 us, 2 tiles 64 us = 525 TFLOP/s, 4 tiles, one wave a SIMD, 80 us).
+  // A tile takes DK / 32 * pieces * 4 registers of queries, DK / 4 of sums and 8 of scores.
   constexpr int PER = DK / 32 * Pieces<T>::Q * 4 + DK / 4 + 8, MOST = 4 * PER <= 120 ? 4 : 2 * PER <= 120 ? 2 : 1;
   const int M = a.G * a.Lq;
   if (M == 1) launch_row<T, DK>(a, s);
@@ -1307,9 +1310,10 @@ extern "C" int tvae_kv8_attn(const void* q, int64_t ldqb, int64_t ldqi, int64_t 
   TVAE_CHECK(lens || (len0 >= 0 && len0 <= (int64_t)per_seq * page), TVAE_E_SHAPE, "tvae_kv8_attn: %d keys do not fit %d pages of %d tokens",
              len0, per_seq, page);
   TVAE_CHECK(!key_mask || (mask_w >= 0 && ld_mask >= mask_w), TVAE_E_SHAPE, "tvae_kv8_attn: bad mask shape");
-  TVAE_CHECK(splits >= 1 && splits <= 1024 && (splits == 1 || ws), TVAE_E_SHAPE, "tvae_kv8_attn: 1 .. 1024 splits, more than one with a workspace");
+  TVAE_CHECK(splits >= 1 && splits <= 1024 && (splits == 1 || (ws && aligned16(ws))), TVAE_E_SHAPE,
+             "tvae_kv8_attn: 1 .. 1024 splits, more than one with a 16-byte aligned workspace");
   const int64_t rows = (int64_t)n * Lq * h * G;
-  TVAE_CHECK((splits > 1 ? rows : (rows + 3) / 4) <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_attn: too many query rows in one call");
+  TVAE_CHECK((splits > 1 ? rows : (rows + 3) / 4) <= MAX_BLOCKS && rows * splits <= 4 * MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_attn: too many query rows in one call");
   if (rows == 0) return TVAE_OK;
   const int64_t cap = lens ? (int64_t)per_seq * page : len0;
   int64_t chunk = ((cap + splits - 1) / splits + 127) / 128 * 128;

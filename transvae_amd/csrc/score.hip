@@ -13,8 +13,9 @@ namespace {
 struct F16 { _Float16 v; };
 struct B16 { uint16_t v; };
 constexpr float LOG2E = 1.44269504088896341f;
+constexpr int SHORT = 256;                                 // classes that 32 lanes hold in registers (8 a lane)
 constexpr int NO_KEY = INT32_MIN;                          // below every value
-constexpr int64_t MAX_BLOCKS = (1 << 22) - 1;              // of up to 1024 threads: a grid counts its threads in 32 bits
+constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;              // of 256 threads: a grid counts its threads in 32 bits
 
 __device__ inline float value_of(float x) { return x; }
 __device__ inline float value_of(B16 x) { return __uint_as_float((uint32_t)x.v << 16); }
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(256) void score_bwd_kernel(ScoreBwdArgs a) {
 // Rows of at most 256 classes: 32 lanes a row; what a class gets of its own is added up in shared memory first.
 template <typename T>
 __global__ __launch_bounds__(256) void score_short_bwd_kernel(ScoreBwdArgs a) {
-  __shared__ float own[8][256];
+  __shared__ float own[8][SHORT];
   const int lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
   const int64_t row = (int64_t)blockIdx.x * 8 + slot;
   const bool live = row < a.rows;
@@ -633,7 +634,7 @@ int type_bytes(int dtype) { return dtype == TVAE_F32 ? 4 : dtype == TVAE_BF16 ||
 
 template <typename T>
 void launch_score(const ScoreArgs& a, hipStream_t s) {
-  if (a.V <= 256) {
+  if (a.V <= SHORT) {
     const dim3 grid((unsigned)((a.rows + 7) / 8)), block(256);
     if (a.V <= 32) hipLaunchKernelGGL((score_short_kernel<T, 1>), grid, block, 0, s, a);
     else if (a.V <= 64) hipLaunchKernelGGL((score_short_kernel<T, 2>), grid, block, 0, s, a);
@@ -648,7 +649,7 @@ void launch_score(const ScoreArgs& a, hipStream_t s) {
 
 template <typename T>
 void launch_bwd(const ScoreBwdArgs& a, hipStream_t s) {
-  if (a.V <= 256) hipLaunchKernelGGL(score_short_bwd_kernel<T>, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, s, a);
+  if (a.V <= SHORT) hipLaunchKernelGGL(score_short_bwd_kernel<T>, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, s, a);
   else hipLaunchKernelGGL(score_bwd_kernel<T>, dim3((unsigned)a.rows, (unsigned)((a.V + a.seg_len - 1) / a.seg_len)), dim3(256), 0, s, a);
 }
 
@@ -665,7 +666,7 @@ extern "C" int tvae_token_logp(const void* logits, int64_t ld, int dtype, const 
   TVAE_CHECK(logits && logp && entropy && (top == 0 || (top_logp && top_ids)), TVAE_E_NULL, "tvae_token_logp: null pointer");
   TVAE_CHECK((uintptr_t)logits % type_bytes(dtype) == 0, TVAE_E_SHAPE, "tvae_token_logp: logits are not aligned to their type");
   TVAE_CHECK(segs >= 1 && segs <= 1024 && (segs == 1 || ws), TVAE_E_SHAPE, "tvae_token_logp: 1 .. 1024 parts, more than one with a workspace");
-  TVAE_CHECK(rows <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_token_logp: too many rows in one call (%lld)", (long long)rows);
+  TVAE_CHECK((V <= SHORT ? (rows + 7) / 8 : rows) <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_token_logp: too many rows in one call (%lld)", (long long)rows);
   const int64_t seg_len = ((V + segs - 1) / segs + 7) / 8 * 8;
   ScoreArgs a = {logits, tokens, logp, entropy, stat, top_logp, ws, top_ids, ld, ld_tok, tok_sub, rows, V, ld_logp, ld_ent, seg_len, top, segs};
   if (dtype == TVAE_F32) launch_score<float>(a, (hipStream_t)stream);
@@ -687,7 +688,7 @@ extern "C" int tvae_token_logp_bwd(const void* logits, int64_t ld, int dtype, co
   TVAE_CHECK(logits && stat && entropy && dx && (!g_top || top == 0 || top_ids), TVAE_E_NULL, "tvae_token_logp_bwd: null pointer");
   TVAE_CHECK((uintptr_t)logits % type_bytes(dtype) == 0 && (uintptr_t)dx % type_bytes(dtype) == 0, TVAE_E_SHAPE,
              "tvae_token_logp_bwd: logits or dx are not aligned to their type");
-  TVAE_CHECK(rows <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_token_logp_bwd: too many rows in one call (%lld)", (long long)rows);
+  TVAE_CHECK((V <= SHORT ? (rows + 7) / 8 : rows) <= MAX_BLOCKS, TVAE_E_SHAPE, "tvae_token_logp_bwd: too many rows in one call (%lld)", (long long)rows);
   const int64_t seg_len = 16384;
   TVAE_CHECK((V + seg_len - 1) / seg_len <= 65535, TVAE_E_SHAPE, "tvae_token_logp_bwd: V too large (%lld)", (long long)V);
   ScoreBwdArgs a = {logits, dx, tokens, top_ids, stat, entropy, g_logp, g_entropy, g_top, ld, ld_tok, tok_sub, rows, V, ld_ent, seg_len,

@@ -224,6 +224,22 @@ class GreedyDecoder:
                     ops.token_logp(logits, ids[:, t + 1], tok_sub=1, out=(logp[:, t], ent[:, t]))
             yield out
 
+    @torch.no_grad()
+    def cache_error(self, z, key_mask):
+        """(layers, 2): what 8 bits do to the memory's keys and values of the latents z, as |rounded - exact| / |exact| (2-norms over
+        the tokens of key_mask), layer by layer.  Stores them as run() would and reads them back."""
+        mem = self.model.decoder.expand_memory(z, ops.MaskSpec(key_mask=key_mask))
+        n, Ls, d = mem.shape
+        seen = (key_mask != 0)[:, :, None, None]
+        out = []
+        for lyr in self.model.decoder.layers:
+            exact = [ops.linear_fwd(mem.reshape(n * Ls, d), lin.weight, lin.bias) for lin in lyr.src_attn.linears[1:3]]
+            cache = self._store8(_cache8(n, Ls, self.h, d // self.h, mem.device), *exact)
+            for got, x in zip(cache.load(Ls), exact):
+                x = x.view(got.shape) * seen
+                out.append(torch.linalg.vector_norm(got * seen - x) / torch.linalg.vector_norm(x))
+        return torch.stack(out).view(-1, 2)
+
     @staticmethod
     def _store8(cache, k, v):
         "k, v (n * tokens, h * dk), projections of every token, into an empty cache"

@@ -92,7 +92,10 @@ class KV8Cache:
     def _ints(self, x, n, name):
         "(address or 0, number): per-sequence int32 values, or one number for all of them"
         if x is None or not torch.is_tensor(x):
-            return 0, 0 if x is None else int(x)
+            x = 0 if x is None else int(x)
+            if not -(1 << 31) <= x < 1 << 31:
+                raise TvaeError("%s must fit 32 bits (got %d)" % (name, x))
+            return 0, x
         if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] != n or not x.is_contiguous():
             raise TvaeError("%s must be a number or a contiguous int32 tensor of %d values, got %s %s" % (name, n, x.dtype, tuple(x.shape)))
         return _ptr(self._on(x, name)), 0
@@ -143,7 +146,7 @@ class KV8Cache:
         `causal` query i sees lens - (Lq - 1 - i) tokens.  key_mask (n, W) bool or uint8: only tokens j < W with a non-zero
         entry.  scale: 1 / sqrt(dk) by default.  A query that sees nothing gets zeros.  q's type is the result's; sums and
         softmax are fp32.  splits: parts that a sequence's tokens are cut into (by a rule of the sizes if None).  A lens tensor's
-        values count at most as many tokens as the pages hold.  Returns `out` (or a new tensor of q's shape)."""
+        values count at most as many tokens as the pages hold.  `out` may be q itself.  Returns `out` (or a new tensor of q's shape)."""
         q = _rows(q, "q")
         n, Lq, hq, dk = q.shape
         if dk != self.dk or hq % self.heads or hq == 0:
@@ -165,6 +168,8 @@ class KV8Cache:
         else:
             if out.shape != q.shape or out.dtype != q.dtype:
                 raise TvaeError("attend: out must have q's shape and type, got %s %s" % (tuple(out.shape), out.dtype))
+            if any(st == 0 and sz > 1 for st, sz in zip(out.stride(), out.shape)):
+                raise TvaeError("attend: out has several elements at one address (strides %s)" % (out.stride(),))
             self._on(out, "out")
             o = _rows(out, "out")
         if splits is None:

@@ -822,7 +822,8 @@ class VAEShell():
         mem = mem.to(dev).float()
         n = mem.shape[0]
         if self.model_type != 'transformer':
-            self._fp32_cache_only(kv_cache)
+            if kv_cache != 'fp32':
+                self._transformer_only("kv_cache=%r" % (kv_cache,))
             return self._rnn_greedy_decode(mem, condition, scores)
         if src_mask is None:
             lens = self.model.encoder.predict_mask_length(mem)            # (n, 1) int64, may be 0
@@ -840,12 +841,28 @@ class VAEShell():
         finally:
             self.model.train(was_training)
 
+    @torch.no_grad()
+    def kv_cache_error(self, mem):
+        """What kv_cache='fp8' does to the keys and values of the latents `mem` (n, d_latent): a (layers, 2) tensor of relative errors
+        of the memory's keys and values, over the tokens that the predicted lengths leave.  For choosing a cache: rounding to
+        3 mantissa bits alone gives 2-3 %; much more means values that one scale for 32 tokens does not span."""
+        self._transformer_only('kv_cache_error')
+        dev = self._device()
+        mem = mem.to(dev).float()
+        lens = self.model.encoder.predict_mask_length(mem)
+        key_mask = (torch.arange(self.src_len + 1, device=dev)[None, :] < lens).to(torch.uint8).contiguous()
+        was_training = self.model.training
+        self.model.eval()
+        try:
+            return GreedyDecoder(self.model, self.params['h'], 'fp8').cache_error(mem, key_mask)
+        finally:
+            self.model.train(was_training)
+
     DECODE_SLAB = 65536     # latents in flight in decode_latents: ~110 GB of K/V caches for trans4x-256
 
-    @staticmethod
-    def _fp32_cache_only(kv_cache):
-        if kv_cache != 'fp32':
-            raise ops._lib.TvaeError("kv_cache=%r: a recurrent model keeps no key/value cache" % (kv_cache,))
+    def _transformer_only(self, what):
+        if self.model_type != 'transformer':
+            raise ops._lib.TvaeError("%s: a recurrent model keeps no key/value cache" % what)
 
     @torch.no_grad()
     def decode_latents(self, mem, condition=[], slab=None, kv_cache='fp32', scores=False):
