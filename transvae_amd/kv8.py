@@ -18,7 +18,8 @@ DK = (32, 64, 128, 256)
 
 
 def _rows(t, name):
-    "t as rows that the kernels take: dense in the last dimension, every row on a 16-byte border (copied only if it is not)"
+    """(t, strides of sequence, token and head): t as rows that the kernels take, dense in the last dimension, every row on a 16-byte
+    border (copied only if it is not)"""
     if t.dim() != 4 or t.dtype not in _TYPES:
         raise TvaeError("%s must be a 4-dimensional float32, bfloat16 or float16 tensor (got %s %s)" % (name, tuple(t.shape), t.dtype))
     a, b, c, one = t.stride()
@@ -26,7 +27,8 @@ def _rows(t, name):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t
+        a, b, c, _ = t.stride()
+    return t, a, b, c
 
 
 class KV8Cache:
@@ -40,16 +42,17 @@ class KV8Cache:
     __slots__ = ("k", "v", "k_exp", "v_exp", "n_seq", "n_pages", "heads", "page", "dk", "device")
 
     def __init__(self, k, v, k_exp, v_exp, n_seq=None):
-        if k.dim() != 4 or v.shape != k.shape or k_exp.shape != k.shape[:2] or v_exp.shape != k_exp.shape:
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or k_exp.shape != (shape[0], shape[1]) or v_exp.shape != (shape[0], shape[1]):
             raise TvaeError("cache: codes must be (n_pages, heads, page, dk) and exponents (n_pages, heads), got %s %s %s %s"
                             % (tuple(k.shape), tuple(v.shape), tuple(k_exp.shape), tuple(v_exp.shape)))
-        dev = k.device
-        for t in (k, v, k_exp, v_exp):
-            if t.dtype is not torch.uint8 or t.device != dev or not t.is_contiguous():
-                raise TvaeError("cache: codes and exponents must be contiguous uint8 tensors of one device")
+        dev, u8 = k.device, torch.uint8
+        if not (k.dtype is u8 and v.dtype is u8 and k_exp.dtype is u8 and v_exp.dtype is u8 and v.device == dev and k_exp.device == dev
+                and v_exp.device == dev and k.is_contiguous() and v.is_contiguous() and k_exp.is_contiguous() and v_exp.is_contiguous()):
+            raise TvaeError("cache: codes and exponents must be contiguous uint8 tensors of one device")
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
-        self.n_pages, self.heads, self.page, self.dk = k.shape
-        self.device = k.device
+        self.n_pages, self.heads, self.page, self.dk = shape
+        self.device = dev
         if self.dk not in DK or self.page < 16 or self.page > 256 or self.page & (self.page - 1):
             raise TvaeError("cache: dk must be one of %s and page a power of two in [16, 256] (got dk %d, page %d)" % (DK, self.dk, self.page))
         if n_seq is not None and (n_seq < 1 or self.n_pages % n_seq):
@@ -112,7 +115,7 @@ class KV8Cache:
         """Rows t < count[b] (None: all) of k, v (n, T, heads, dk) become tokens start[b] + t of sequence b.  `start` and
         `count` are numbers or int32 (n,) tensors on the device.  Overwriting from the middle of a sequence leaves what
         stands behind it dead; no page may belong to two sequences of one call.  k and v are not differentiated."""
-        k, v = _rows(k, "k"), _rows(v, "v")
+        (k, *ks), (v, *vs) = _rows(k, "k"), _rows(v, "v")
         n, T = k.shape[:2]
         if v.shape != k.shape or v.dtype != k.dtype or tuple(k.shape[2:]) != (self.heads, self.dk):
             raise TvaeError("store: k and v must both be (n, T, %d, %d) of one type, got %s %s and %s %s"
@@ -123,7 +126,7 @@ class KV8Cache:
             T, count = min(T, max(0, int(count))), None
         sp, s0 = self._ints(start, n, "start")
         cp, _ = self._ints(count, n, "count")
-        self._call("tvae_kv8_store", _ptr(k), *k.stride()[:3], _ptr(v), *v.stride()[:3], _TYPES[k.dtype], *self._cache_args(), tab, per,
+        self._call("tvae_kv8_store", _ptr(k), *ks, _ptr(v), *vs, _TYPES[k.dtype], *self._cache_args(), tab, per,
                    sp, s0, cp, n, T, self.heads, self.dk, self.page)
 
     def load(self, T, start=0, count=None, table=None, dtype=torch.float32):
@@ -147,7 +150,7 @@ class KV8Cache:
         entry.  scale: 1 / sqrt(dk) by default.  A query that sees nothing gets zeros.  q's type is the result's; sums and
         softmax are fp32.  splits: parts that a sequence's tokens are cut into (by a rule of the sizes if None).  A lens tensor's
         values count at most as many tokens as the pages hold.  `out` may be q itself.  Returns `out` (or a new tensor of q's shape)."""
-        q = _rows(q, "q")
+        q, qa, qb, qc = _rows(q, "q")
         n, Lq, hq, dk = q.shape
         if dk != self.dk or hq % self.heads or hq == 0:
             raise TvaeError("attend: q must be (n, Lq, G * %d, %d), got %s" % (self.heads, self.dk, tuple(q.shape)))
@@ -164,20 +167,21 @@ class KV8Cache:
             ldm = max(key_mask.stride(0), mw)
             mp = _ptr(self._on(key_mask, "key_mask") if mw else self.k_exp)             # no column: nothing is visible, nothing is read
         if out is None:
-            o = out = torch.empty((n, Lq, hq, dk), dtype=q.dtype, device=q.device)
+            o = out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            oa, ob, oc = Lq * hq * dk, hq * dk, dk
         else:
             if out.shape != q.shape or out.dtype != q.dtype:
                 raise TvaeError("attend: out must have q's shape and type, got %s %s" % (tuple(out.shape), out.dtype))
             if any(st == 0 and sz > 1 for st, sz in zip(out.stride(), out.shape)):
                 raise TvaeError("attend: out has several elements at one address (strides %s)" % (out.stride(),))
             self._on(out, "out")
-            o = _rows(out, "out")
+            o, oa, ob, oc = _rows(out, "out")
         if splits is None:
             splits = self._splits(n, hq // self.heads * Lq, per * self.page if lp else l0)
         ws = None
         if splits > 1:
             ws = torch.empty(n * Lq * hq * splits * (dk + 2), dtype=torch.float32, device=q.device)
-        self._call("tvae_kv8_attn", _ptr(q), *q.stride()[:3], _ptr(o), *o.stride()[:3], _TYPES[q.dtype], *self._cache_args(), tab, per,
+        self._call("tvae_kv8_attn", _ptr(q), qa, qb, qc, _ptr(o), oa, ob, oc, _TYPES[q.dtype], *self._cache_args(), tab, per,
                    lp, l0, mp, ldm, mw, int(causal), n, self.heads, hq // self.heads, Lq, dk, self.page,
                    1.0 / math.sqrt(dk) if scale is None else float(scale), splits, _ptr(ws))
         if o is not out:

@@ -1300,7 +1300,7 @@ LOGIT_TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 def _logit_rows(logits):
     "(rows, V) view of the logits, dense in the class dimension (copied only if it is not), and its row stride"
     V = logits.shape[-1]
-    lg = logits.reshape(-1, V)
+    lg = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if (V > 1 and lg.stride(1) != 1) or (lg.shape[0] > 1 and lg.stride(0) < V):
         lg = lg.contiguous()
     return lg, lg.stride(0) if lg.shape[0] > 1 else V
