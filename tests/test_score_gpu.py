@@ -187,6 +187,28 @@ def test_same_row_whatever_stands_beside_it():
         assert torch.equal(u, v) and torch.allclose(u[:3].double(), w.double(), rtol=1e-6, atol=1e-6)
 
 
+def test_many_rows_a_wave_each():
+    "from 4096 rows on a wave has a row of its own: the same values as in small calls, ties and masked classes included"
+    from transvae_amd.loss import token_logprobs
+    x = torch.randn((4100, 3000), generator=torch.Generator().manual_seed(8)).to(torch.bfloat16)
+    x[5] = 1.0
+    x[6] = -math.inf
+    x[7, 1:] = -math.inf
+    x[8, 2999] = math.nan
+    x[9] = torch.arange(3000).float() / 16
+    y = torch.arange(4100) % 3001 - 1
+    a = token_logprobs(x.cuda(), y.cuda(), top=20)
+    check(x[:12], y[:12], 20, grads=False)
+    b = token_logprobs(x[:64].cuda(), y[:64].cuda(), top=20)
+    assert torch.equal(a[3][:64], b[3])
+    for u, w in zip(a[:3], b[:3]):
+        assert torch.equal(torch.isnan(u[:64]), torch.isnan(w)) and torch.allclose(u[:64].nan_to_num(0, 0, 0), w.nan_to_num(0, 0, 0), rtol=1e-6, atol=2e-6)
+    wl, we, wt, wi = score(x[-30:], y[-30:], 20)
+    assert torch.equal(a[3][-30:].cpu(), wi)
+    close(a[0][-30:], wl, value_bound(x, wl))
+    close(a[2][-30:], wt, value_bound(x, wt))
+
+
 def test_offsets_past_two_gigabytes():
     "rows * V over 2^31 elements: the last rows are those of a small call"
     from transvae_amd.loss import token_logprobs
