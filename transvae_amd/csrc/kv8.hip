@@ -395,10 +395,10 @@ struct LoadArgs {
   int start0, T, h, page;
 };
 
-// A thread makes four times 16 bytes of the result (4 or 8 values), a block's width apart and all in flight together; tokens of
-// one head lie next to each other: a page's rows of a head are read in order, and what a wave writes are whole rows.  The
-// result is written past the caches: kept in them it only delays the end of the launch (measured at 500 x 127 x 4 x 64 fp32:
-// 40 us through the caches, 27 us past them).
+// A thread makes four times 16 bytes of the result (4 or 8 values), a block's width apart and all in flight together.  Blocks go
+// through the result in its own order: writes are three quarters of the traffic and more, and are whole runs of all heads (24 x 4000
+// x 8 x 128 bf16: 118 us so, 128 us in the order of the pages).  The result is written past the caches: kept in them it only
+// delays the end of the launch (500 x 127 x 4 x 64 fp32: 40 us through the caches, 25 us past them).
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void kv8_load_kernel(LoadArgs a) {
   constexpr int N = 16 / sizeof(T), LPR = DK / N, U = 4;
@@ -411,11 +411,11 @@ __global__ __launch_bounds__(256) void kv8_load_kernel(LoadArgs a) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t i = i0 + 256 * u < a.total ? i0 + 256 * u : 0;
-    const uint32_t row = i / LPR, bh = a.by_T.div(row);
+    const uint32_t row = i / LPR, bt = a.by_h.div(row);
     sub[u] = i % LPR;
-    t[u] = row - bh * a.T;
-    b[u] = a.by_h.div(bh);
-    head[u] = bh - b[u] * a.h;
+    head[u] = row - bt * a.h;
+    b[u] = a.by_T.div(bt);
+    t[u] = bt - b[u] * a.T;
     pos[u] = (int64_t)(a.start ? a.start[b[u]] : a.start0) + t[u];
     const int cnt = a.count ? a.count[b[u]] : a.T;
     const bool live = (int)t[u] < cnt && pos[u] >= 0 && (pos[u] >> shift) < a.pages.per_seq;
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256) void kv8_load_kernel(LoadArgs a) {
 #pragma unroll
       for (int v = 0; v < 4; ++v) Elem<T>::put(out + k + v, y[v] * s);
     }
-    T* o = reinterpret_cast<T*>(a.out[side]) + (((size_t)b[u] * a.T + t[u]) * a.h + head[u]) * DK + N * sub[u];
+    T* o = reinterpret_cast<T*>(a.out[side]) + (size_t)(i0 + 256 * u) * N;
     __builtin_nontemporal_store(*reinterpret_cast<const uintx4*>(out), reinterpret_cast<uintx4*>(o));
   }
 }
