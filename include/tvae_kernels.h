@@ -452,7 +452,7 @@ int tvae_kv8_attn(const void* q, int64_t ldqb, int64_t ldqi, int64_t ldqh, void*
  * counterpart in the reference, whose losses give weighted means only, transvae/loss.py:8-38).  Row r: logits + r * ld, V
  * values of dtype TVAE_F32, TVAE_BF16 or TVAE_F16, any alignment; class y = tokens[r * ld_tok] - tok_sub (tokens NULL or y
  * outside [0, V): no token, logp 0).  With M = max x, L = ln sum exp(x - M):
- *   logp[r * ld_logp] = x_y - M - L ; entropy[r * ld_ent] = L - sum exp(x - M) (x - M) / e^L ; stat (rows, 2) = {M, L}
+ *   logp[r * ld_logp] = x_y - M - L ; entropy[r * ld_ent] = L - sum exp(x - M) (x - M) / e^L ; stat (rows, 2) = {M, L}, or NULL
  *   top_ids, top_logp (rows, top): by descending logit, then ascending class (NaN above +inf)
  * A row of -inf only: logp and top_logp -inf, entropy 0.  A NaN or +inf makes the row's values NaN.
  * segs (1 .. 1024): rows are cut into that many parts, joined by a second launch over ws, rows * segs * (3 + 2 top) floats

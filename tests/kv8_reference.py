@@ -140,9 +140,16 @@ def attend_bound(o, wv, qk, dk, keys, dtype):
     return rel[..., None] * wv + half * o.abs() + torch.finfo(dtype).smallest_normal
 
 
+def _shifted(logits):
+    "the logits in float64 less their row's maximum, which changes no probability: 1e38 + ln V is 1e38 in 64 bits too"
+    x = logits.double()
+    top = x.nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf).amax(1, keepdim=True)
+    return x - torch.where(torch.isfinite(top), top, torch.zeros_like(top))
+
+
 def score(logits, tokens, top):
     "(logp, entropy, top_logp, top_ids) in float64"
-    x = logits.double()
+    x = _shifted(logits)
     rows, V = x.shape
     lse = torch.logsumexp(x, 1)
     lp = x - lse[:, None]
@@ -157,6 +164,7 @@ def score(logits, tokens, top):
         ok = (tokens >= 0) & (tokens < V)
         logp[ok] = lp[ok, tokens[ok]]
     ids = torch.zeros((rows, top), dtype=torch.int64)
+    x = logits.double()
     for r in range(rows):
         order = sorted(range(V), key=lambda c: (0 if math.isnan(x[r, c]) else 1, 0.0 if math.isnan(x[r, c]) else -float(x[r, c]), c))
         ids[r] = torch.tensor(order[:top], dtype=torch.int64)
@@ -165,7 +173,7 @@ def score(logits, tokens, top):
 
 def score_grad(logits, tokens, ids, g_logp, g_ent, g_top):
     "gradient of sum(g_logp logp) + sum(g_ent H) + sum(g_top top_logp), from the formula"
-    x = logits.double()
+    x = _shifted(logits)
     rows, V = x.shape
     lse = torch.logsumexp(x, 1)
     lp = x - lse[:, None]

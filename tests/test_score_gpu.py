@@ -107,6 +107,30 @@ def test_nan_and_infinity_stay_in_their_row(V):
     check(x, torch.tensor([-1] * 6), 3, grads=False)
 
 
+@pytest.mark.parametrize("V", [20, 700, 9001])
+def test_masks_of_the_lowest_value_beside_huge_logits(V):
+    "differences that leave fp32's range weigh nothing, and nothing becomes NaN"
+    for dtype in (torch.float32, torch.bfloat16):
+        low = torch.finfo(dtype).min
+        x = torch.randn((5, V), generator=torch.Generator().manual_seed(V)).to(dtype)
+        x[0, ::2] = low
+        x[1, 1:] = low
+        x[1, 0] = 3e38
+        x[2, :] = low
+        x[3, V // 2:] = low
+        x[3, :V // 2] = 2e31
+        x[4, 3] = -low
+        from transvae_amd.loss import token_logprobs
+        xg = x.cuda().requires_grad_()
+        logp, ent, tl, ti = token_logprobs(xg, torch.tensor([1, 0, 2, 0, 3]).cuda(), top=2)
+        wl, we, wt, wi = score(x, torch.tensor([1, 0, 2, 0, 3]), 2)
+        assert torch.equal(ti.cpu(), wi)
+        close(logp, wl, value_bound(x, wl))
+        close(ent, we, value_bound(x, we) + 1e-6)
+        g, = torch.autograd.grad(logp.sum() + ent.sum() + tl.sum(), xg)
+        assert bool(torch.isfinite(g).all())
+
+
 def test_zeros_of_both_signs_tie():
     x = torch.full((2, 40), -1.0)
     x[0, 7], x[0, 3] = 0.0, -0.0

@@ -70,7 +70,7 @@ struct Sums {
     l += e;
     t = fmaf(e, fmaxf(d, -1e30f), t);                      // -inf adds 0, not 0 * inf
   }
-  __device__ inline void add_finite(float x) {             // m and x are finite, m at least x; a NaN passes too
+  __device__ inline void add_finite(float x) {             // x - m is finite (x > -inf, x <= m < 1e30), or x is NaN
     const float d = x - m, e = __builtin_amdgcn_exp2f(d * LOG2E);
     l += e;
     t = fmaf(e, d, t);
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
         if (i0 + (H + h) * STEP + lane < body) ahead[h] = *reinterpret_cast<const uint4*>(xv + i0 + (H + h) * STEP + lane);
       const float both = fmaxf(vm[0], vm[H - 1]);
       if (both > s.m) s.grow(both);
-      if (__all(least > -INFINITY && s.m < INFINITY && s.m > -INFINITY)) {    // masked classes want more care: -inf adds 0, not 0 * inf
+      if (__all(least > -INFINITY && s.m < 1e30f && s.m > -INFINITY)) {       // else more care: -inf, or a difference that overflows to it, adds 0, not 0 * inf
 #pragma unroll
         for (int h = 0; h < H; ++h) {
 #pragma unroll
