@@ -456,7 +456,7 @@ int tvae_kv8_attn(const void* q, int64_t ldqb, int64_t ldqi, int64_t ldqh, void*
  *   top_ids, top_logp (rows, top): by descending logit, then ascending class (NaN above +inf)
  * A row of -inf only: logp and top_logp -inf, entropy 0.  A NaN or +inf makes the row's values NaN.
  * segs (1 .. 1024): rows are cut into that many parts, joined by a second launch over ws, rows * segs * (3 + 2 top) floats
- * (segs 1: NULL).
+ * aligned to 8 bytes (segs 1: NULL).
  *   bwd: dx (rows, V) contiguous, of the logits' type, from the forward's stat, entropy and top_ids and the gradients
  *   g_logp (rows), g_entropy (rows), g_top (rows, top), each of which may be NULL; every element of dx is written:
  *   dx_j = g_logp (d_jy - p_j) - g_entropy p_j (ln p_j + H) + sum_t g_top_t (d_{j, top_t} - p_j); 0 where the logit is -inf.

@@ -138,6 +138,28 @@ def test_zeros_of_both_signs_tie():
     check(x, None, 4)
 
 
+@pytest.mark.parametrize("rows,V", [(1, 4099), (2, 30001), (1, 100003), (1, 149999)])
+@pytest.mark.parametrize("top", [1, 8, 20, 64])
+def test_equal_logits_and_bests_in_one_place_of_long_rows(rows, V, top):
+    "long rows are cut into parts: more equal values than a block has threads, all the best in one part, in the last one, none at all"
+    g = torch.Generator().manual_seed(V + top)
+    for kind in range(6):
+        x = torch.randn((rows, V), generator=g)
+        if kind == 0:
+            x[:] = 0.5
+        elif kind == 1:
+            x[:] = -math.inf
+        elif kind == 2:
+            x[:, V // 2:V // 2 + 100] += 20.0
+        elif kind == 3:
+            x[:, -70:] = 9.0
+        elif kind == 4:
+            x = x.sort(dim=1).values
+        else:
+            x = (x * 2).round()                                    # few different values
+        check(x, torch.arange(rows) * 37 + V // 2, top, grads=False)
+
+
 def test_strides_phases_and_leading_dimensions():
     from transvae_amd.loss import token_logprobs
     g = torch.Generator().manual_seed(1)
