@@ -298,3 +298,32 @@ def test_streams_and_replayed_graphs():
                 gr.replay()
                 torch.cuda.synchronize()
                 assert all(torch.equal(u, w) for u, w in zip(out, token_logprobs(x, y, top=5)))
+
+
+def test_captured_gradients_replay():
+    "the capture comes before any eager gradient of the same leaf is alive, as for every backward pass"
+    from transvae_amd.loss import token_logprobs
+    for rows, V, dtype in ((500, 25, torch.float32), (3, 30001, torch.float16), (700, 3001, torch.bfloat16)):
+        x = torch.randn((rows, V), generator=torch.Generator().manual_seed(V)).to(dtype).cuda().requires_grad_()
+        y = (torch.arange(rows) % V).cuda()
+        gl, ge, gt = torch.randn(rows).cuda(), torch.randn(rows).cuda(), torch.randn((rows, 3)).cuda()
+
+        def step():
+            logp, ent, tl, _ = token_logprobs(x, y, top=3)
+            return torch.autograd.grad((logp, ent, tl), x, (gl, ge, gt))[0]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            dx = step()
+        for rep in range(4):
+            with torch.no_grad():
+                x.copy_(torch.randn((rows, V), generator=torch.Generator().manual_seed(rep)))
+            gl.normal_(), gt.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(dx, step())

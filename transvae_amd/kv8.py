@@ -32,7 +32,7 @@ def _rows(t, name):
 
 
 class KV8Cache:
-    """Keys and values of some sequences in 8 bits.
+    """Keys and values of some sequences in 8 bits.  For serving: nothing here is differentiated.
 
     ``KV8Cache.empty(n_pages, heads, dk, page)`` makes a pool whose pages block tables hand out;
     ``KV8Cache.for_batch(n, max_len, heads, dk, page)`` one whose pages belong to `n` sequences in order (no tables).
@@ -114,7 +114,7 @@ class KV8Cache:
     def store(self, k, v, start=0, count=None, table=None):
         """Rows t < count[b] (None: all) of k, v (n, T, heads, dk) become tokens start[b] + t of sequence b.  `start` and
         `count` are numbers or int32 (n,) tensors on the device.  Overwriting from the middle of a sequence leaves what
-        stands behind it dead; no page may belong to two sequences of one call.  k and v are not differentiated."""
+        stands behind it dead; no page may stand twice in the tables of one call."""
         (k, *ks), (v, *vs) = _rows(k, "k"), _rows(v, "v")
         n, T = k.shape[:2]
         if v.shape != k.shape or v.dtype != k.dtype or tuple(k.shape[2:]) != (self.heads, self.dk):
@@ -149,7 +149,8 @@ class KV8Cache:
         `causal` query i sees lens - (Lq - 1 - i) tokens.  key_mask (n, W) bool or uint8: only tokens j < W with a non-zero
         entry.  scale: 1 / sqrt(dk) by default.  A query that sees nothing gets zeros.  q's type is the result's; sums and
         softmax are fp32.  splits: parts that a sequence's tokens are cut into (by a rule of the sizes if None).  A lens tensor's
-        values count at most as many tokens as the pages hold.  `out` may be q itself.  Returns `out` (or a new tensor of q's shape)."""
+        values count at most as many tokens as the pages hold.  `out` may be q itself, but overlap
+        it in no other way.  Returns `out` (or a new tensor of q's shape)."""
         q, qa, qb, qc = _rows(q, "q")
         n, Lq, hq, dk = q.shape
         if dk != self.dk or hq % self.heads or hq == 0:
