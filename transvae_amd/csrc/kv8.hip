@@ -1217,7 +1217,10 @@ void launch_load(const LoadArgs& a, int dk, hipStream_t s) {
 }
 template <typename T, int DK>
 void launch_row(const AttnArgs& a, hipStream_t s) {
-  if (a.rows * a.splits >= 8192)
+  // a wave a row where the rows fill the chip, else a block a row: rows of different lengths then even out (wave / block, 0 .. keys
+  // tokens a row, DK = 64: 2048 rows of 128 keys 10.6 / 12.1 us, of 2048 68 / 53; 8064 rows of 128 17 / 31 us, of 512 50 / 52, of
+  // 2048 203 / 182; DK = 256, 4096 rows of 64 19 / 20, of 256 56 / 48)
+  if (a.rows * a.splits >= (int64_t)a.chunk * DK / 4 || a.rows > MAX_BLOCKS)
     hipLaunchKernelGGL((kv8_attn_row_kernel<T, DK, 1>), dim3((unsigned)((a.rows + 3) / 4), a.splits), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((kv8_attn_row_kernel<T, DK, 4>), dim3((unsigned)a.rows, a.splits), dim3(256), 0, s, a);
@@ -1225,7 +1228,11 @@ void launch_row(const AttnArgs& a, hipStream_t s) {
 template <typename T, int DK, int NT>
 void launch_tile(const AttnArgs& a, hipStream_t s) {
   const int64_t tiles = (a.G * a.Lq + 16 * NT - 1) / (16 * NT), groups = (int64_t)a.n * a.h * a.splits, units = groups * tiles;
-  if (units >= 8192)
+  // a wave a unit where units fill the chip or keys are few, else a block a unit, whose waves have to meet at the end (wave / block,
+  // 0 .. keys tokens a sequence, 4 query heads a key head, bf16: DK = 128, 4096 units of 128 keys 26 / 51 us, of 1024 118 / 109, of
+  // 2048 214 / 190; DK = 256, where a block has its compute unit to itself, 1024 units of 128 keys 15 / 42, of 1024 60 / 79, of 4096
+  // 223 / 209; 132 rows a key head, DK = 64: 1536 units of 512 keys 37 / 46, of 2048 95 / 87)
+  if (units >= (int64_t)a.chunk * (DK == 256 ? 1 : 3) || units + 8 * tiles > MAX_BLOCKS)
     hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 4>), dim3((unsigned)((groups + 7) / 8 * 8 * tiles)), dim3(256), 0, s, a);
