@@ -197,6 +197,49 @@ def test_attend_matches_the_definition(case, dtype):
             assert bool((off <= lim).all()), (causal, scale, float((off / lim).max()), (off / lim).argmax())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,h,per,Lq,G,dk,page,splits", [
+    (2, 2, 20, 1, 4, 64, 32, 1), (2, 2, 20, 5, 2, 128, 32, 3), (110, 4, 4, 1, 4, 32, 32, 1), (40, 10, 7, 2, 1, 64, 16, 1),
+    (3, 1, 5, 3, 1, 256, 64, 2), (70, 2, 8, 1, 1, 32, 16, 1), (9, 2, 3, 1, 1, 64, 128, 1)])
+def test_masks_of_runs(n, h, per, Lq, G, dk, page, splits, dtype):
+    "runs of masked tokens longer and shorter than what a kernel takes at once, single visible tokens, none; NaN codes behind the masks"
+    gpu, ref, tab, rtab = pair(n, per, h, dk, page, True, seed=43)
+    fill(gpu, ref)
+    W = per * page
+    g = torch.Generator().manual_seed(47)
+    mask = torch.zeros((n, W + 5), dtype=torch.bool)
+    for b in range(n):
+        kind = b % 6
+        if kind == 0:
+            mask[b, W // 2:W // 2 + 40] = True
+        elif kind == 1:
+            mask[b, int(torch.randint(0, W, (1,), generator=g))] = True
+        elif kind == 2:
+            mask[b] = True
+            mask[b, 16:16 + 48] = False
+        elif kind == 3:
+            mask[b] = True
+            mask[b, 5:min(W - 3, 75)] = False
+        elif kind == 4:
+            mask[b] = (torch.arange(W + 5) // 16) % 2 == 1
+    if n > 50:
+        rtab[1, per - 1] = -1
+        tab.copy_(rtab.cuda())
+    lens = [W - (b * 7) % 23 for b in range(n)]
+    q = (torch.randn((n, Lq, h * G, dk), generator=g) * 0.2).to(dtype)
+    clean = ref.attend(q, lens, rtab, per, True, mask)
+    for b in range(n):
+        for i in range(per):
+            p = ref.page_of(rtab, per, b, i)
+            if p is not None:
+                dead = ~mask[b, i * page:(i + 1) * page].cuda()
+                gpu.k[p][:, dead] = 127
+                gpu.v[p][:, dead] = 255
+    o = gpu.attend(q.cuda(), ints(lens), table=tab, key_mask=mask.cuda(), splits=splits)
+    lim = attend_bound(*clean, dk, W, dtype)
+    assert bool(((o.cpu().double() - clean[0]).abs() <= lim).all())
+
+
 @pytest.mark.parametrize("Lq,G", [(1, 1), (1, 4), (9, 2)])
 def test_what_is_dead_or_masked_never_matters(Lq, G):
     "NaN codes and exponents of 255 in dead rows, masked tokens, pages of nobody; absent pages"

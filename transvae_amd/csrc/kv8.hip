@@ -806,7 +806,7 @@ __device__ inline void value_frag(Frag& f, const uint32_t (&v)[8][CodeTile<DK>::
 // the eight token rows of V into columns), nothing is staged in shared memory.  The running maximum is only raised when a
 // score passes it by 2^8: until then weights just exceed 1, which costs no precision and saves the rescaling.
 // KW = 4: the block's waves take every fourth group of 32 tokens and meet at the end; KW = 1: every wave has rows of its own.
-template <typename T, int DK, int NT, int KW>
+template <typename T, int DK, int NT, int KW, bool MASKED>
 __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv8_attn_tile_kernel(AttnArgs a) {
   constexpr int W = DK / 16, KS = DK / 32, NQ = Pieces<T>::Q, NP = Pieces<T>::P, VW = CodeTile<DK>::VW, VG = W < 4 ? W : 4;
   constexpr int REGS = NT * (4 * W + 2);
@@ -878,19 +878,33 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv8_attn_tile_kernel(A
   int64_t t0 = beg + 32 * kw;
   auto ask = [&](int64_t tok) { return pages.ask(tok < most ? (int)(tok >> shift) : 0); };
   auto page = [&](int raw, int64_t tok) { return pages.page(raw, (int)(tok >> shift), tok < most); };
+  // the mask of 32 tokens: a byte a lane, then a bit each
+  const uint8_t* mk = a.mask + (MASKED ? (int64_t)b * a.ld_mask : 0);
+  auto ask_mask = [&](int64_t tok) {
+    const int64_t j = tok + (lane & 31);
+    return MASKED ? (int)mk[j < a.mask_w ? j : 0] : 1;
+  };
+  auto mask_bits = [&](int raw, int64_t tok) { return MASKED ? (uint32_t)__ballot(raw != 0 && tok + (lane & 31) < a.mask_w) : ~0u; };
   const uint32_t koff = c * DK + (DK == 32 ? 8 : 16) * quad, voff = 4 * quad * DK + W * c;
   bool strange = false;
-  // page ids (the same for all lanes) are looked up two groups ahead, codes loaded one group ahead; where there is no page, page 0
-  // is read instead
+  // page ids (the same for all lanes) and masks are looked up two groups ahead, codes loaded one group ahead; where there is no page,
+  // or 16 tokens are masked, page 0 is read instead, and a group with nothing else is passed over
   CodeTile<DK> tile0, tile1;
-  int ra = ask(t0), rb = ask(t0 + 16);
-  int id0 = page(ra, t0), id1 = page(rb, t0 + 16);
-  ra = ask(t0 + step), rb = ask(t0 + step + 16);
+  int ra = ask(t0), rb = ask(t0 + 16), rm = ask_mask(t0);
+  uint32_t bits = mask_bits(rm, t0);
+  int id0 = bits & 0xFFFF ? page(ra, t0) : -1, id1 = bits >> 16 ? page(rb, t0 + 16) : -1;
+  ra = ask(t0 + step), rb = ask(t0 + step + 16), rm = ask_mask(t0 + step);
   tile0.load(a, head, id0 < 0 ? 0 : id0, id1 < 0 ? 0 : id1, t0, koff, voff);
   auto group_of_32 = [&](CodeTile<DK>& cur, CodeTile<DK>& nxt) {
-    const int nd0 = page(ra, t0 + step), nd1 = page(rb, t0 + step + 16);
-    ra = ask(t0 + 2 * step), rb = ask(t0 + 2 * step + 16);
+    const uint32_t next_bits = mask_bits(rm, t0 + step);
+    const int nd0 = next_bits & 0xFFFF ? page(ra, t0 + step) : -1, nd1 = next_bits >> 16 ? page(rb, t0 + step + 16) : -1;
+    ra = ask(t0 + 2 * step), rb = ask(t0 + 2 * step + 16), rm = ask_mask(t0 + 2 * step);
     nxt.load(a, head, nd0 < 0 ? 0 : nd0, nd1 < 0 ? 0 : nd1, t0 + step, koff, voff);
+    if (MASKED && id0 < 0 && id1 < 0) {
+      id0 = nd0, id1 = nd1, bits = next_bits;
+      t0 += step;
+      return;
+    }
     // raw scores: sc[t][i][e] is the lane's query c of tile t against token t0 + 16 i + 4 quad + e
     floatx4 sc[NT][2];
 #pragma unroll
@@ -917,21 +931,10 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv8_attn_tile_kernel(A
     }
     const float ks[2] = {exp_scale(cur.ek[0]) * scale, exp_scale(cur.ek[1]) * scale};
     float vs[2] = {exp_scale(cur.ev[0]), exp_scale(cur.ev[1])};
-    const bool plain = t0 + 32 <= least && !a.mask && id0 >= 0 && id1 >= 0;      // every row of the unit sees all 32 tokens
+    const bool plain = t0 + 32 <= least && bits == ~0u && id0 >= 0 && id1 >= 0;  // every row of the unit sees all 32 tokens
     if (!plain) {
-      uint32_t seen = (id0 >= 0 ? 0x0Fu : 0u) | (id1 >= 0 ? 0xF0u : 0u);         // bit i: the lane's i-th token exists and is not masked
-      if (a.mask) {
-        const uint8_t* mk = a.mask + (int64_t)b * a.ld_mask;
-        uint8_t mb[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int64_t j = t0 + token_of(i, quad);
-          mb[i] = mk[j < a.mask_w ? j : 0];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (t0 + token_of(i, quad) >= a.mask_w || mb[i] == 0) seen &= ~(1u << i);
-      }
+      // bit i: the lane's i-th token exists and is not masked
+      const uint32_t seen = (id0 >= 0 ? bits >> 4 * quad & 0x0Fu : 0u) | (id1 >= 0 ? (bits >> (16 + 4 * quad) & 0x0Fu) << 4 : 0u);
       // codes that no row sees must not be NaN (0 * NaN is not 0); nor may those that only some rows see: they are taken out
       // here and put back behind the loop.  Half a page that nobody sees may hold any exponent.
       const bool some = least < most && t0 + 32 > least;
@@ -1005,7 +1008,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv8_attn_tile_kernel(A
         }
       }
     }
-    id0 = nd0, id1 = nd1;
+    id0 = nd0, id1 = nd1, bits = next_bits;
     t0 += step;
   };
   while (t0 < most) {
@@ -1018,7 +1021,7 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv8_attn_tile_kernel(A
       if (g0 + 32 <= least) continue;
       for (int64_t j = g0; j < g0 + 32 && j < most; ++j) {
         const int id = page(ask(j), j);
-        if (id < 0 || (a.mask && (j >= a.mask_w || a.mask[(int64_t)b * a.ld_mask + j] == 0))) continue;
+        if (id < 0 || (MASKED && (j >= a.mask_w || mk[j] == 0))) continue;
         const uint8_t* p = a.codes[1] + (((size_t)id * a.h + head) * a.page + ((int)j & pm)) * DK + 4 * W * quad;
 #pragma unroll
         for (int i = 0; i < 4 * W; ++i) {                               // dimension W e + g of the lane's 4 W
@@ -1225,17 +1228,24 @@ void launch_row(const AttnArgs& a, hipStream_t s) {
   else
     hipLaunchKernelGGL((kv8_attn_row_kernel<T, DK, 4>), dim3((unsigned)a.rows, a.splits), dim3(256), 0, s, a);
 }
-template <typename T, int DK, int NT>
-void launch_tile(const AttnArgs& a, hipStream_t s) {
+template <typename T, int DK, int NT, bool MASKED>
+void launch_tile_as(const AttnArgs& a, hipStream_t s) {
   const int64_t tiles = (a.G * a.Lq + 16 * NT - 1) / (16 * NT), groups = (int64_t)a.n * a.h * a.splits, units = groups * tiles;
   // a wave a unit where units fill the chip or keys are few, else a block a unit, whose waves have to meet at the end (wave / block,
   // 0 .. keys tokens a sequence, 4 query heads a key head, bf16: DK = 128, 4096 units of 128 keys 26 / 51 us, of 1024 118 / 109, of
   // 2048 214 / 190; DK = 256, where a block has its compute unit to itself, 1024 units of 128 keys 15 / 42, of 1024 60 / 79, of 4096
   // 223 / 209; 132 rows a key head, DK = 64: 1536 units of 512 keys 37 / 46, of 2048 95 / 87)
   if (units >= (int64_t)a.chunk * (DK == 256 ? 1 : 3) || units + 8 * tiles > MAX_BLOCKS)
-    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 1, MASKED>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 4>), dim3((unsigned)((groups + 7) / 8 * 8 * tiles)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 4, MASKED>), dim3((unsigned)((groups + 7) / 8 * 8 * tiles)), dim3(256), 0, s, a);
+}
+// masks are a variant of their own: looked up two groups ahead, a byte a lane and a ballot, they cost 2 to 5 % (23 sequences of 15 k tokens,
+// 99 rows a key head, DK = 256, all visible: 532 -> 269 us against eight byte loads a lane where they are needed)
+template <typename T, int DK, int NT>
+void launch_tile(const AttnArgs& a, hipStream_t s) {
+  if (a.mask) launch_tile_as<T, DK, NT, true>(a, s);
+  else launch_tile_as<T, DK, NT, false>(a, s);
 }
 template <typename T, int DK>
 void launch_dk(const AttnArgs& a, hipStream_t s) {
