@@ -221,10 +221,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
   constexpr int NV = Vec<T>::N, H = 8 / NV;
   __shared__ float sums[W == 1 ? 4 : W][3];
   __shared__ int2 cand[W == 1 ? 4 : W][64];
-  // W > 1: each wave's `share`-th best key so far.  W shares are `top` values, so `top` values of the row reach the least of
+  // W > 1: each full wave's `share`-th best key so far.  The shares are `top` values, so `top` values of the row reach the least of
   // them; a stale one is only lower, so the waves do not wait for each other to read them
   __shared__ int pub[4];
-  const int share = (a.top + W - 1) / W;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   const int kw = W == 1 ? 0 : wave;
@@ -240,6 +239,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
     int64_t head = ((16 - ((uintptr_t)(x + c0) & 15)) & 15) / sizeof(T);              // values up to a 16-byte border
     if (head > c1 - c0) head = c1 - c0;
     const int64_t body = (c1 - c0 - head) / NV, tail = c0 + head + body * NV;
+    // waves that begin with 64 vectors share the bar; one with fewer would hold it down (2745 classes in two parts: 76 us with it)
+    const int full = W == 1 || body < 128 ? 1 : body < W * 64 ? (int)(body >> 6) : W;
+    const int share = (a.top + full - 1) / full;
     // Enters what of v[0 .. N) (lane o's values are classes base + o * N ..) can be among the best.  `own`: the last entry of the
     // wave's list; what equals it is a higher class than all entries and stays out.  `floor`: a key that at least `top` values of
     // the row reach; what equals it may still count.
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
         }
       }
       own = top.entry(a.top - 1);
-      if (W > 1) {
+      if (W > 1 && kw < full) {
         const int q = top.entry(share - 1);
         if (lane == 0 && q != NO_KEY) __hip_atomic_store(&pub[wave], q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
@@ -340,7 +342,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void score_kernel(ScoreArgs 
       }
       if (a.top) {
         if (opening) {                                     // every wave of the block comes by here once
-          const int q = nth_key(key_of(both), lane, share);
+          const int q = kw < full ? nth_key(key_of(both), lane, share) : INT32_MAX;
           if (W > 1) {
             if (lane == 0) __hip_atomic_store(&pub[wave], q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             __syncthreads();
