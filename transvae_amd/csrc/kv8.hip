@@ -303,10 +303,12 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(StoreArgs a) {
 }
 
 // Many rows a sequence: TPU threads per (sequence, touched page, head), K or V.  A thread keeps its first KEEP 16-byte pieces in
-// registers as they came, so the rows are read once; a wave a page where that suffices, a block of four else.
-template <typename T, int DK, int TPU>
+// registers as they came, so the rows are read once; a wave a page where eight of them suffice, a block of four else.  KEEP follows
+// the page: pieces that are never there cost their instructions and registers all the same (264 x 968 rows of 5 heads: 16 x 32
+// bf16 a page, 1 / 16 pieces 64 / 166 us; 32 x 64 fp32, 8 / 16 165 / 222; 64 x 128 bf16, four waves with 4 / one with 16 179 / 213).
+template <typename T, int DK, int TPU, int KEEP>
 __global__ __launch_bounds__(256) void kv8_store_kernel(StoreArgs a) {
-  constexpr int N = Raw<T>::N, LPR = DK / N, RPI = TPU / LPR, KEEP = 16;        // values a piece, lanes a row, rows a step
+  constexpr int N = Raw<T>::N, LPR = DK / N, RPI = TPU / LPR;                   // values a piece, lanes a row, rows a step
   __shared__ uint32_t red[4];
   const int tid = threadIdx.x % TPU, side = blockIdx.y;
   uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * (256 / TPU) + threadIdx.x / TPU);
@@ -1200,8 +1202,12 @@ template <typename T, int DK>
 void launch_store_dk(const StoreArgs& a, int units, hipStream_t s) {
   constexpr int N = Raw<T>::N;
   if (a.T <= 4) hipLaunchKernelGGL((kv8_append_kernel<T, DK>), dim3(cdiv(units, 256 * N / DK)), dim3(256), 0, s, a);
-  else if (a.page * DK <= 64 * 16 * N) hipLaunchKernelGGL((kv8_store_kernel<T, DK, 64>), dim3(cdiv(units, 4), 2), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((kv8_store_kernel<T, DK, 256>), dim3(units, 2), dim3(256), 0, s, a);
+  else if (a.page * DK <= 64 * N) hipLaunchKernelGGL((kv8_store_kernel<T, DK, 64, 1>), dim3(cdiv(units, 4), 2), dim3(256), 0, s, a);
+  else if (a.page * DK <= 64 * 4 * N) hipLaunchKernelGGL((kv8_store_kernel<T, DK, 64, 4>), dim3(cdiv(units, 4), 2), dim3(256), 0, s, a);
+  else if (a.page * DK <= 64 * 8 * N) hipLaunchKernelGGL((kv8_store_kernel<T, DK, 64, 8>), dim3(cdiv(units, 4), 2), dim3(256), 0, s, a);
+  else if (a.page * DK <= 256 * 4 * N) hipLaunchKernelGGL((kv8_store_kernel<T, DK, 256, 4>), dim3(units, 2), dim3(256), 0, s, a);
+  else if (a.page * DK <= 256 * 8 * N) hipLaunchKernelGGL((kv8_store_kernel<T, DK, 256, 8>), dim3(units, 2), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((kv8_store_kernel<T, DK, 256, 16>), dim3(units, 2), dim3(256), 0, s, a);
 }
 template <typename T>
 void launch_store(const StoreArgs& a, int dk, int units, hipStream_t s) {
