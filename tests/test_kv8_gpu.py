@@ -102,6 +102,21 @@ def test_store_rounds_as_defined(dtype, n, T, h, dk, page, start, count, paged):
     same_cache(gpu, ref)                                           # every page: what was not written stays
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dk", [32, 64, 128, 256])
+def test_pages_of_every_size(dtype, dk, page):
+    "a thread keeps as many pieces as the page needs: whole pages, one that has rows in front, one that ends early"
+    n, h, per, T = 2, 2, 3, 2 * page - 3
+    gpu, ref, tab, rtab = pair(n, per, h, dk, page, False, seed=dk + page)
+    g = torch.Generator().manual_seed(page)
+    for start, size in ((0, 1.0), (page // 2 + 1, 40.0)):
+        k, v = ((torch.randn((n, T, h, dk), generator=g) * size).to(dtype) for _ in range(2))
+        gpu.store(k.cuda(), v.cuda(), start=start)
+        ref.store(k, v, [start] * n, [T] * n, rtab, per)
+        same_cache(gpu, ref)
+
+
 def test_store_ties_ends_and_what_has_no_code():
     "halves go to the even code; the page's scale at its borders; zeros, denormals, the largest floats, infinities and NaN"
     h, dk, page = 4, 32, 16
