@@ -102,6 +102,10 @@ def test_token_logp_refuses(bad):
     assert _fwd(**bad) < 0 and _lib().lib().tvae_last_error()
 
 
+def test_token_logp_refuses_a_workspace_off_its_border():
+    assert _fwd(segs=2, ws=C.c_void_p(4100)) < 0 and b"aligned to 8" in _lib().lib().tvae_last_error()
+
+
 @pytest.mark.parametrize("bad", SHAPE + [dict(dx=None), dict(ti=None), dict(dx=C.c_void_p(4098))])
 def test_token_logp_bwd_refuses(bad):
     assert _bwd(**bad) < 0 and _lib().lib().tvae_last_error()
