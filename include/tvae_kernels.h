@@ -431,6 +431,8 @@ int tvae_gather_batch(const uint8_t* ids, int64_t ld_ids, const float* props, co
  *     j < lens[b] (lens NULL: len0), with causal != 0 only j < lens[b] - (Lq - 1 - i) for query token i; key_mask (n, ld_mask)
  *     or NULL: only j < mask_w with a non-zero byte.  A query that sees no key gets zeros (unlike tvae_decode_attn, whose
  *     -1e9 fill lets it attend uniformly).  What stands in masked or dead places never matters, NaN included.
+ *     Scores, softmax and sums are fp32; with 16-bit q and Lq * G > 1 each weight is rounded to within 2^-17 of itself where it meets
+ *     the values (their sum takes the unrounded ones).
  *     splits: the tokens are cut into that many parts (1 .. 1024), joined by a second launch over the workspace
  *     ws of n * Lq * h * G * splits * (dk + 2) floats (splits 1: NULL).
  */

@@ -1,0 +1,80 @@
+"""Attention over the 8-bit cache against a vectorised 64-bit form, for what the loops of tests/kv8_reference.py are too slow to reach:
+the precision of its parts, and the kernel variants that only many rows select."""
+import math
+
+import pytest
+import torch
+
+from kv8_reference import VALUES, attend_bound
+
+pytestmark = pytest.mark.gpu
+
+
+def cache_of(pages, h, dk, page, n_seq, seed):
+    "random codes without NaN and exponents around 1, made on the GPU"
+    from transvae_amd.kv8 import KV8Cache
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    c = KV8Cache.empty(pages, h, dk, page, "cuda:0", n_seq=n_seq)
+    for name in ("k", "v"):
+        codes = torch.randint(0, 256, c.k.shape, generator=gen, device="cuda", dtype=torch.uint8)
+        codes[(codes & 127) == 127] = 126
+        getattr(c, name).copy_(codes)
+        getattr(c, name + "_exp").copy_(torch.randint(117, 122, c.k_exp.shape, generator=gen, device="cuda", dtype=torch.uint8))
+    return c
+
+
+def attend64(c, q, lens, table=None, causal=True, mask=None, scale=None):
+    "what tests/kv8_reference.py's Cache.attend gives, on the GPU and some sequences at a time; lens (n,) on the GPU"
+    n, Lq, hq, dk = q.shape
+    h, page = c.heads, c.page
+    per = c.n_pages // c.n_seq if table is None else table.shape[1]
+    ids = torch.arange(n * per, device="cuda").view(n, per) if table is None else table.long()
+    L, G = per * page, hq // h
+    scale = 1 / math.sqrt(dk) if scale is None else scale
+    values = VALUES.cuda()
+    out = [torch.empty(q.shape, dtype=torch.float64, device="cuda") for _ in range(2)] + [torch.empty((n, Lq, hq), dtype=torch.float64, device="cuda")]
+    some = max(1, (1 << 24) // (L * h * max(dk, Lq * G)))
+    for a in range(0, n, some):
+        b = slice(a, min(n, a + some))
+        B = b.stop - a
+        there = (ids[b] >= 0) & (ids[b] < c.n_pages)
+        at = torch.where(there, ids[b], torch.zeros_like(ids[b]))
+        k, v = (torch.where(there[:, :, None, None, None], values[x[at].long()] * torch.exp2(e[at].double() - 127)[..., None, None], 0.0)
+                .transpose(1, 2).reshape(B, h, L, dk).contiguous() for x, e in ((c.k, c.k_exp), (c.v, c.v_exp)))
+        qh = q[b].double().view(B, Lq, h, G, dk).permute(0, 2, 1, 3, 4).reshape(B, h, Lq * G, dk).contiguous()
+        j, i = torch.arange(L, device="cuda"), torch.arange(Lq, device="cuda")
+        ll = lens[b].long().clamp(0, L)
+        see = j < (ll[:, None, None] - (Lq - 1 - i if causal else 0 * i)[None, :, None])
+        see = see & there.repeat_interleave(page, 1)[:, None]
+        if mask is not None:
+            seen = torch.zeros((B, L), dtype=torch.bool, device="cuda")
+            w = min(L, mask.shape[1])
+            seen[:, :w] = mask[b, :w] != 0
+            see = see & seen[:, None]
+        see = see[:, None, :, None].expand(B, h, Lq, G, L).reshape(B, h, Lq * G, L)
+        kt = k.transpose(2, 3).contiguous()
+        s = (torch.matmul(qh, kt) * scale).masked_fill(~see, -math.inf)
+        qk = (torch.matmul(qh.abs(), kt.abs()) * abs(scale)).masked_fill(~see, 0.0).amax(-1)
+        w = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+        back = lambda x: x.view(B, h, Lq, G, -1).permute(0, 2, 1, 3, 4).reshape(B, Lq, hq, -1)
+        out[0][b], out[1][b], out[2][b] = back(torch.matmul(w, v)), back(torch.matmul(w, v.abs())), back(qk[..., None])[..., 0]
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Lq,G", [(1, 4), (9, 2), (5, 8)])
+@pytest.mark.parametrize("dk", [32, 64, 128, 256])
+def test_weights_of_16_bit_queries_are_not_rounded_to_16_bits(dk, Lq, G, dtype):
+    """Keys in pairs that differ in one dimension, their values in sign only: what is left of a pair is the difference of two close
+    weights, a few thousandths of them, so the result's own rounding is as much smaller and shows how the weights were rounded.
+    They may be off by 2^-17 relative; the rest is attend_bound's for fp32."""
+    n, h, page, per = 2, 2, 32, 3
+    c = cache_of(n * per, h, dk, page, n, dk)
+    c.k[:, :, 1::2, 1:] = c.k[:, :, ::2, 1:]
+    c.v[:, :, 1::2] = c.v[:, :, ::2] ^ 128
+    q = (torch.randn((n, Lq, h * G, dk), generator=torch.Generator().manual_seed(Lq)) * 0.05).to(dtype).cuda()
+    lens = torch.tensor([96, 70], dtype=torch.int32).cuda()
+    want, wv, qk = attend64(c, q, lens, causal=False)
+    lim = attend_bound(want, wv, qk, dk, per * page, torch.float32) + 2.0 ** -17 * wv + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal
+    off = (c.attend(q, lens, causal=False).double() - want).abs()
+    assert bool((off <= lim).all()), float((off / lim).max())

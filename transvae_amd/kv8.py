@@ -148,7 +148,8 @@ class KV8Cache:
         every sequence (a number or an int32 (n,) tensor).  The Lq queries are the LAST tokens of what lens counts: with
         `causal` query i sees lens - (Lq - 1 - i) tokens.  key_mask (n, W) bool or uint8: only tokens j < W with a non-zero
         entry.  scale: 1 / sqrt(dk) by default.  A query that sees nothing gets zeros.  q's type is the result's; sums and
-        softmax are fp32.  splits: parts that a sequence's tokens are cut into (by a rule of the sizes if None).  A lens tensor's
+        softmax are fp32 (with several 16-bit queries a key head, Lq * G > 1, each weight is rounded to within 2^-17 where it meets
+        the values; their sum is not).  splits: parts that a sequence's tokens are cut into (by a rule of the sizes if None).  A lens tensor's
         values count at most as many tokens as the pages hold.  `out` may be q itself, but overlap
         it in no other way.  Returns `out` (or a new tensor of q's shape)."""
         q, qa, qb, qc = _rows(q, "q")
