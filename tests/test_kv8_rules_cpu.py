@@ -1,0 +1,21 @@
+"""Rules of the 8-bit cache and of the token scores that need no GPU."""
+import pytest
+import torch
+
+
+def _cache(heads=1, pages=2):
+    from transvae_amd.kv8 import KV8Cache
+    k, v = (torch.zeros((pages, heads, 16, 32), dtype=torch.uint8) for _ in range(2))
+    return KV8Cache(k, v, *(torch.zeros((pages, heads), dtype=torch.uint8) for _ in range(2)))
+
+
+@pytest.mark.parametrize("heads", [1, 2, 3, 8, 40])
+def test_parts_stay_within_what_the_kernel_takes(heads):
+    "1 .. 1024 parts and rows * parts within one launch, whatever the sequences, queries and capacity"
+    c = _cache(heads)
+    for n in (0, 1, 2, 7, 255, 256, 2047, 70000):
+        for rows in (0, 1, 16, 17, 500):
+            for keys in (0, 1, 255, 1024, 100000, 1 << 20, (1 << 20) + 16, 1 << 21, (1 << 31) - 1):
+                parts = c._splits(n, rows, keys)
+                assert 1 <= parts <= 1024, (n, rows, keys, parts)
+                assert parts == 1 or n * rows * heads * parts <= 4 * ((1 << 24) - 1), (n, rows, keys, parts)

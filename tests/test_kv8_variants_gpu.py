@@ -78,3 +78,15 @@ def test_weights_of_16_bit_queries_are_not_rounded_to_16_bits(dk, Lq, G, dtype):
     lim = attend_bound(want, wv, qk, dk, per * page, torch.float32) + 2.0 ** -17 * wv + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal
     off = (c.attend(q, lens, causal=False).double() - want).abs()
     assert bool((off <= lim).all()), float((off / lim).max())
+
+
+@pytest.mark.parametrize("G,Lq", [(1, 1), (4, 3)])
+def test_a_million_tokens_and_a_table_of_as_many(G, Lq):
+    "the default number of parts stays within what the join takes; a part sums at most 1152 keys, the join 1024 parts"
+    h, dk, page, L = 1, 32, 256, (1 << 20) + 256 * 100
+    c = cache_of(L // page, h, dk, page, 1, 3)
+    q = (torch.randn((1, Lq, G, dk), generator=torch.Generator().manual_seed(1)) * 0.2).cuda()
+    for lens in (L, torch.tensor([L - 5], dtype=torch.int32).cuda(), torch.tensor([300], dtype=torch.int32).cuda()):
+        want, wv, qk = attend64(c, q, torch.as_tensor([lens]).cuda() if isinstance(lens, int) else lens)
+        off = (c.attend(q, lens).double() - want).abs()
+        assert bool((off <= attend_bound(want, wv, qk, dk, 1152 + 1024, torch.float32)).all())

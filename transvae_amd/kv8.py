@@ -197,4 +197,5 @@ class KV8Cache:
         # enough blocks for the 256 compute units with parts of 256 tokens and more, and up to 2048 with parts of 1024 and more,
         # so that sequences of different lengths even out (one of 131 k tokens, 2 key heads: 64 parts 29 us, 128 21 us, 256 24 us;
         # 48 ragged ones up to 8 k, 8 key heads: 1 part 191 us, 5 parts 96 us)
-        return max(1, min(-(-keys // 1024), 2048 // units), min(-(-keys // 256), 256 // units))
+        # (one sequence and head reach 2048 only past a million tokens: 1024 is what one join takes)
+        return max(1, min(-(-keys // 1024), 2048 // units, 1024), min(-(-keys // 256), 256 // units))
