@@ -19,3 +19,12 @@ def test_parts_stay_within_what_the_kernel_takes(heads):
                 parts = c._splits(n, rows, keys)
                 assert 1 <= parts <= 1024, (n, rows, keys, parts)
                 assert parts == 1 or n * rows * heads * parts <= 4 * ((1 << 24) - 1), (n, rows, keys, parts)
+
+
+def test_nothing_to_do_needs_no_workspace():
+    "no sequences or no queries, with several parts: a workspace of no elements has no address"
+    import ctypes as C
+    from transvae_amd import _lib
+    P = C.c_void_p(4096)
+    for n, Lq in ((0, 1), (2, 0)):
+        assert _lib.lib().tvae_kv8_attn(P, 64, 64, 64, P, 64, 64, 64, 0, P, P, P, P, 8, None, 4, None, 5, None, 0, 0, 1, n, 1, 1, Lq, 64, 32, 1.0, 3, None, None) == 0

@@ -90,3 +90,12 @@ def test_a_million_tokens_and_a_table_of_as_many(G, Lq):
         want, wv, qk = attend64(c, q, torch.as_tensor([lens]).cuda() if isinstance(lens, int) else lens)
         off = (c.attend(q, lens).double() - want).abs()
         assert bool((off <= attend_bound(want, wv, qk, dk, 1152 + 1024, torch.float32)).all())
+
+
+@pytest.mark.parametrize("Lq,n", [(0, 1), (1, 0)])
+def test_nothing_to_attend_over_long_sequences(Lq, n):
+    "no queries or no sequences, where the tokens would be cut into parts"
+    c = cache_of(8, 1, 32, 256, None, 5)
+    table = torch.arange(8, dtype=torch.int32).cuda().view(1, 8)[:n]
+    for splits in (None, 3):
+        assert c.attend(torch.zeros((n, Lq, 1, 32)).cuda(), 2048, table=table, splits=splits).shape == (n, Lq, 1, 32)

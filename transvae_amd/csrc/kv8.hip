@@ -1342,9 +1342,9 @@ extern "C" int tvae_kv8_attn(const void* q, int64_t ldqb, int64_t ldqi, int64_t 
   TVAE_CHECK(lens || (len0 >= 0 && len0 <= (int64_t)per_seq * page), TVAE_E_SHAPE, "tvae_kv8_attn: %d keys do not fit %d pages of %d tokens",
              len0, per_seq, page);
   TVAE_CHECK(!key_mask || (mask_w >= 0 && ld_mask >= mask_w), TVAE_E_SHAPE, "tvae_kv8_attn: bad mask shape");
-  TVAE_CHECK(splits >= 1 && splits <= 1024 && (splits == 1 || (ws && aligned16(ws))), TVAE_E_SHAPE,
-             "tvae_kv8_attn: 1 .. 1024 splits, more than one with a 16-byte aligned workspace");
   const int64_t rows = (int64_t)n * Lq * h * G;
+  TVAE_CHECK(splits >= 1 && splits <= 1024 && (splits == 1 || rows == 0 || (ws && aligned16(ws))), TVAE_E_SHAPE,
+             "tvae_kv8_attn: 1 .. 1024 splits, more than one with a 16-byte aligned workspace");
   TVAE_CHECK((splits > 1 ? rows : (rows + 3) / 4) <= MAX_BLOCKS && rows * splits <= 4 * MAX_BLOCKS, TVAE_E_SHAPE, "tvae_kv8_attn: too many query rows in one call");
   if (rows == 0) return TVAE_OK;
   const int64_t cap = lens ? (int64_t)per_seq * page : len0;
