@@ -28,3 +28,15 @@ def test_nothing_to_do_needs_no_workspace():
     P = C.c_void_p(4096)
     for n, Lq in ((0, 1), (2, 0)):
         assert _lib.lib().tvae_kv8_attn(P, 64, 64, 64, P, 64, 64, 64, 0, P, P, P, P, 8, None, 4, None, 5, None, 0, 0, 1, n, 1, 1, Lq, 64, 32, 1.0, 3, None, None) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_have_strides_that_the_kernels_take(dtype):
+    "dimensions of one element keep any stride: a slice of one token out of an odd-width buffer too"
+    from transvae_amd.kv8 import _rows
+    for shape in ((1, 1, 1, 65), (1, 1, 3, 65), (1, 2, 1, 67), (2, 1, 1, 65), (1, 1, 1, 64), (2, 3, 2, 72)):
+        base = torch.arange(float(torch.Size(shape).numel())).view(shape).to(dtype)
+        t = base[..., :64]
+        r, *ld = _rows(t, "t")
+        assert all(x * r.element_size() % 16 == 0 for x in ld) and r.data_ptr() % 16 == 0
+        assert torch.equal(torch.as_strided(r, r.shape, (*ld, 1), r.storage_offset()), t)

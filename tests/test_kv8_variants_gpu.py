@@ -99,3 +99,16 @@ def test_nothing_to_attend_over_long_sequences(Lq, n):
     table = torch.arange(8, dtype=torch.int32).cuda().view(1, 8)[:n]
     for splits in (None, 3):
         assert c.attend(torch.zeros((n, Lq, 1, 32)).cuda(), 2048, table=table, splits=splits).shape == (n, Lq, 1, 32)
+
+
+def test_one_token_out_of_an_odd_width_buffer():
+    "one sequence, one token, one head: strides of single elements are no strides"
+    c, d = (cache_of(2, 1, 64, 16, 1, 7) for _ in range(2))
+    g = torch.Generator().manual_seed(1)
+    k, v, q, out = (torch.randn((1, 1, 1, 65), generator=g).cuda()[..., :64] for _ in range(4))
+    dense = lambda x: x.clone(memory_format=torch.contiguous_format).view(64).view(1, 1, 1, 64)
+    c.store(k, v, start=9)
+    d.store(dense(k), dense(v), start=9)
+    assert all(torch.equal(getattr(c, x), getattr(d, x)) for x in ("k", "v", "k_exp", "v_exp"))
+    want = c.attend(dense(q), 10)
+    assert torch.equal(c.attend(q, 10), want) and c.attend(q, 10, out=out) is out and torch.equal(out, want)

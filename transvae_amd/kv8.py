@@ -27,7 +27,8 @@ def _rows(t, name):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        a, b, c, _ = t.stride()
+        _, T, h, dk = t.shape
+        a, b, c = T * h * dk, h * dk, dk               # not t.stride(): a dimension of one element keeps any stride
     return t, a, b, c
 
 
