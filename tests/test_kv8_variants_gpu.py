@@ -112,3 +112,55 @@ def test_one_token_out_of_an_odd_width_buffer():
     assert all(torch.equal(getattr(c, x), getattr(d, x)) for x in ("k", "v", "k_exp", "v_exp"))
     want = c.attend(dense(q), 10)
     assert torch.equal(c.attend(q, 10), want) and c.attend(q, 10, out=out) is out and torch.equal(out, want)
+
+
+def compare(n, h, G, Lq, dk, page, per, dtype, masked, splits=None, causal=True, seed=11):
+    """Ragged sequences (none, one token, all of them), scattered pages, an absent one; codes that no query sees are NaN"""
+    keys = per * page
+    c = cache_of(n * per + 2, h, dk, page, None, seed)
+    g = torch.Generator().manual_seed(seed)
+    table = torch.randperm(n * per + 2, generator=g)[:n * per].view(n, per).to(torch.int32)
+    table[n // 2, per - 1] = -1
+    lens = torch.randint(0, keys + 1, (n,), generator=g, dtype=torch.int32)
+    lens[:4] = torch.tensor([0, 1, keys, keys - 1])[:n]
+    table, lens = table.cuda(), lens.cuda()
+    mask = None
+    if masked:
+        mask = (torch.rand((n, keys - 3), generator=g) < 0.6).cuda()
+        mask[n - 1] = False
+        mask[n - 2, 16:80] = False
+    q = (torch.randn((n, Lq, h * G, dk), generator=g) * 0.2).to(dtype).cuda()
+    want, wv, qk = attend64(c, q, lens, table, causal, mask)
+    live = torch.arange(keys, device="cuda")[None] < lens[:, None]
+    if masked:
+        live[:, :keys - 3] &= mask
+        live[:, keys - 3:] = False
+    there = (table >= 0) & (table < c.n_pages)
+    pages, dead = table[there].long(), ~live.view(n, per, page)[there]
+    for x in (c.k, c.v):
+        x[pages] = torch.where(dead[:, None, :, None], torch.full((), 255, dtype=torch.uint8, device="cuda"), x[pages])
+    off = (c.attend(q, lens, table=table, causal=causal, key_mask=mask, splits=splits).double() - want).abs()
+    lim = attend_bound(want, wv, qk, dk, keys, dtype)
+    assert bool((off <= lim).all()), (float((off / lim).nan_to_num(nan=math.inf).max()), (~(off <= lim)).nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("n,h,dk,page,per,splits", [
+    (257, 4, 32, 16, 8, None), (513, 4, 64, 32, 4, None), (1025, 4, 128, 64, 2, None), (1025, 8, 256, 128, 1, None), (3001, 3, 32, 16, 33, None),
+    (400, 3, 32, 16, 16, 2), (700, 3, 64, 256, 1, 3)])
+def test_single_query_rows_a_wave_each(n, h, dk, page, per, splits, masked, dtype):
+    "so many rows (rows * parts >= keys a part * dk / 4) that a wave takes a row of its own, as in a large decoding step"
+    compare(n, h, 1, 1, dk, page, per, dtype, masked, splits)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Lq,G", [(1, 4), (5, 5), (35, 2), (1, 33)])
+@pytest.mark.parametrize("dk", [32, 64, 128, 256])
+def test_tiles_a_wave_each_and_a_block_each(dk, Lq, G, dtype):
+    """One, two and several tiles of 16 to 64 query rows a key head: 384 tiles of at most 128 keys and more take a wave each (at 256
+    dimensions 128), fewer a block each; masked and not, whole and in parts"""
+    for masked in (False, True):
+        compare(129, 3, G, Lq, dk, 32, 4, dtype, masked)
+        compare(3, 2, G, Lq, dk, 64, 9, dtype, masked)
+    compare(80, 3, G, Lq, dk, 16, 13, dtype, True, splits=2, causal=False)
