@@ -32,6 +32,12 @@ def build_lib(force=False, verbose=False):
     os.makedirs(LIBDIR, exist_ok=True)
     headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_common.h"),
                os.path.join(HERE, "..", "include", "tvae_kernels.h")]
+    # objects made with other flags are stale too: the flags of all of them stand in one file, which is not there while they are made
+    stamp, flags = os.path.join(LIBDIR, "flags.txt"), " ".join(FLAGS)
+    if not os.path.exists(stamp) or open(stamp).read() != flags:
+        force = True
+        if os.path.exists(stamp):
+            os.remove(stamp)
     objs, jobs = [], []
     for src in SOURCES:
         sp = os.path.join(CSRC, src)
@@ -54,6 +60,9 @@ def build_lib(force=False, verbose=False):
                 print(err)
     if jobs or force or _stale(LIB, objs):
         run([_hipcc(), "-shared", "-o", LIB] + objs + ["--offload-arch=gfx950", "-pthread"])
+    if force:
+        with open(stamp, "w") as f:
+            f.write(flags)
     return LIB
 
 
