@@ -40,3 +40,18 @@ def test_rows_have_strides_that_the_kernels_take(dtype):
         r, *ld = _rows(t, "t")
         assert all(x * r.element_size() % 16 == 0 for x in ld) and r.data_ptr() % 16 == 0
         assert torch.equal(torch.as_strided(r, r.shape, (*ld, 1), r.storage_offset()), t)
+
+
+def test_token_logprobs_refuses_forward_mode_derivatives():
+    "a tangent would vanish without a word; refused before anything is launched, with and without a gradient asked for"
+    import torch.autograd.forward_ad as fwad
+    from transvae_amd._lib import TvaeError
+    from transvae_amd.loss import token_logprobs
+    for needs in (False, True):
+        x = torch.zeros(3, 9, requires_grad=needs)
+        with fwad.dual_level():
+            dual = fwad.make_dual(x, torch.ones(3, 9))
+            with pytest.raises(TvaeError, match="forward"):
+                token_logprobs(dual)
+            with pytest.raises(TvaeError, match="host tensor"):        # no tangent: on to the next check
+                token_logprobs(x)

@@ -1,5 +1,6 @@
 """Loss functions with the reference's names (transvae/loss.py), computed by the fused HIP kernel."""
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -42,9 +43,9 @@ def token_logprobs(logits, tokens=None, top=0):
     padding: its logp is 0 and passes no gradient, entropy and alternatives are the row's all the same.  Alternatives come in
     descending order, equal logits in ascending order of their ids.  A class at -inf has probability 0 (and gradient 0); a
     row of nothing else has logp -inf, entropy 0 and gradient 0; a NaN or +inf makes its row NaN.  Results are float32 (ids
-    int64).  logp, entropy and top_logp are differentiable in the logits, once; a captured backward pass is to be captured while no
-    eager autograd graph of the same leaves is alive, as with any other op.  No counterpart in the reference, whose losses
-    (transvae/loss.py:8-38) only give weighted means."""
+    int64).  logp, entropy and top_logp are differentiable in the logits, once and backward (forward-mode tangents
+    are refused); a captured backward pass is to be captured while no eager autograd graph of the same leaves is alive, as with
+    any other op.  No counterpart in the reference, whose losses (transvae/loss.py:8-38) only give weighted means."""
     if logits.dim() < 1 or logits.shape[-1] < 1 or logits.dtype not in ops.LOGIT_TYPES:
         raise ops._lib.TvaeError("token_logprobs: logits must be float32, bfloat16 or float16 (..., V), got %s %s" % (tuple(logits.shape), logits.dtype))
     V, lead = logits.shape[-1], logits.shape[:-1]
@@ -56,6 +57,8 @@ def token_logprobs(logits, tokens=None, top=0):
                                      % (tuple(lead), logits.device, tuple(tokens.shape), tokens.dtype, tokens.device))
         if tokens.dim() != 1 or tokens.dtype != torch.int64:
             tokens = tokens.reshape(-1).long()
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise ops._lib.TvaeError("token_logprobs: no forward-mode derivatives (its gradient is a backward pass)")
     if logits.requires_grad and torch.is_grad_enabled():
         logp, entropy, top_logp, top_ids = ops.TokenLogpFn.apply(logits, tokens, int(top))
     else:
