@@ -596,6 +596,8 @@ struct ScoreBwdArgs {
   int top;
 };
 
+constexpr float NO_WEIGHT = -128.f;                        // e^-128 is 0 in fp32: below it ln p only has to stay finite when g_H multiplies it
+
 // One read and one write a value: p = exp((x - M) - L), dx = -p (pull + g_H (ln p + H)) with pull = g_l + sum g_t; the few
 // classes that are the token or an alternative get their own gradient on top, added by the thread that holds the class.
 template <typename T>
@@ -629,7 +631,7 @@ __global__ __launch_bounds__(256) void score_bwd_kernel(ScoreBwdArgs a) {
   auto grad = [&](float v) {
     const float lp = (v - M) - L;
     const float p = __builtin_amdgcn_exp2f(lp * LOG2E);
-    const float r = -p * (pull + gh * (fmaxf(lp, -1e30f) + H));
+    const float r = -p * (pull + gh * (fmaxf(lp, NO_WEIGHT) + H));
     return none || v == -INFINITY ? 0.f : r;
   };
   int64_t head = ((16 - ((uintptr_t)(x + c0) & 15)) & 15) / sizeof(T);
@@ -696,7 +698,7 @@ __global__ __launch_bounds__(256) void score_short_bwd_kernel(ScoreBwdArgs a) {
   T* dx = reinterpret_cast<T*>(a.dx) + row * a.V;
   for (int c = lane; c < a.V; c += 32) {
     const float v = value_of(x[c]), lp = (v - M) - L, p = __builtin_amdgcn_exp2f(lp * LOG2E);
-    const float r = own[slot][c] - p * (pull + gh * (fmaxf(lp, -1e30f) + H));
+    const float r = own[slot][c] - p * (pull + gh * (fmaxf(lp, NO_WEIGHT) + H));
     put(dx + c, none || v == -INFINITY ? 0.f : r);
   }
 }
