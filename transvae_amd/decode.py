@@ -237,7 +237,8 @@ class GreedyDecoder:
             cache = self._store8(_cache8(n, Ls, self.h, d // self.h, mem.device), *exact)
             for got, x in zip(cache.load(Ls), exact):
                 x = x.view(got.shape) * seen
-                out.append(torch.linalg.vector_norm(got * seen - x) / torch.linalg.vector_norm(x))
+                size = torch.linalg.vector_norm(x)
+                out.append(torch.where(size == 0, size, torch.linalg.vector_norm(got * seen - x) / size))    # no token: no error
         return torch.stack(out).view(-1, 2)
 
     @staticmethod
