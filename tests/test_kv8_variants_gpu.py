@@ -164,3 +164,16 @@ def test_tiles_a_wave_each_and_a_block_each(dk, Lq, G, dtype):
         compare(129, 3, G, Lq, dk, 32, 4, dtype, masked)
         compare(3, 2, G, Lq, dk, 64, 9, dtype, masked)
     compare(80, 3, G, Lq, dk, 16, 13, dtype, True, splits=2, causal=False)
+
+
+def test_a_number_of_rows_may_be_any_number():
+    "count as a number, in store and load alike: none below zero, all of them beyond what there are, also past 32 bits"
+    c, d = (cache_of(4, 2, 64, 16, 2, 7) for _ in range(2))
+    rows = torch.randn((2, 5, 2, 64), generator=torch.Generator().manual_seed(3)).cuda()
+    for count, n in ((1 << 40, 5), (7, 5), (3, 3), (0, 0), (-1, 0), (-(1 << 40), 0)):
+        c.store(rows, rows, start=2, count=count)
+        if n:
+            d.store(rows[:, :n], rows[:, :n], start=2)
+        assert torch.equal(c.k, d.k) and torch.equal(c.v_exp, d.v_exp)
+        k, v = c.load(5, start=2, count=count)
+        assert torch.equal(k[:, :n], d.load(5, start=2)[0][:, :n]) and float(k[:, n:].abs().sum() + v[:, n:].abs().sum()) == 0

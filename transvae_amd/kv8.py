@@ -138,7 +138,7 @@ class KV8Cache:
         tab, per, n = self._pages(table, None)
         sp, s0 = self._ints(start, n, "start")
         if count is not None and not torch.is_tensor(count):
-            count = torch.full((n,), int(count), dtype=torch.int32, device=self.device)
+            count = torch.full((n,), min(T, max(0, int(count))), dtype=torch.int32, device=self.device)
         cp, _ = self._ints(count, n, "count")
         k, v = (torch.empty((n, T, self.heads, self.dk), dtype=dtype, device=self.device) for _ in range(2))
         self._call("tvae_kv8_load", *self._cache_args(), tab, per, sp, s0, cp, _ptr(k), _ptr(v), _TYPES[dtype], n, T, self.heads, self.dk, self.page)
