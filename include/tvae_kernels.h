@@ -421,7 +421,8 @@ int tvae_gather_batch(const uint8_t* ids, int64_t ld_ids, const float* props, co
  * aligned; ld*b, ld*t (or ld*i), ld*h are the strides in elements of sequence, token and head.
  *
  *   store: rows t < min(T, count[b]) (count NULL: T) of k, v (n, T, h, dk) become tokens start[b] + t (start NULL: start0 + t).
- *     Tokens past the last page are dropped, a negative start stores nothing.  The exponent of a (page, head) is the smallest e
+ *     Tokens past the last page are dropped (with start and count NULL start0 + T has to fit), a negative start[b] stores nothing.
+ *     The exponent of a (page, head) is the smallest e
  *     with |x| 2^-e <= 448 over the page's new rows; where rows stand in front of them in the page it is no smaller than the
  *     page's old one, and when it grows those rows are rounded again to the new scale.  What stands behind the new rows in
  *     the page is left as it is and counts as dead.  Infinities and NaN are stored as NaN and do not count for the exponent.

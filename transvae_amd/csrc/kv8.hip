@@ -826,8 +826,9 @@ __global__ __launch_bounds__(256, DK == 256 ? 1 : 2) void kv8_attn_tile_kernel(A
   const int M = a.G * a.Lq, mt = (M + 16 * NT - 1) / (16 * NT);
   const int kw = KW == 1 ? 0 : wave;
   // KW == 4: the tiles of one (sequence, key head, part) read the same codes, so they go to one die, one behind the other: blocks
-  // are dealt to the eight dies in turn, and each has a cache of its own (12 sequences of 4000 tokens, 4 key heads, 7 tiles each,
-  // 3 parts: 68 us with the tiles on different dies, 61 us so)
+  // are dealt to the eight dies in turn, and each has a cache of its own (8 sequences of 60000 tokens, 8 key heads x 128, 64 rows
+  // a key head: with the tiles on different dies 293 us in bf16 and 528 in fp32, 266 and 421 us so; no difference where all codes fit
+  // the memory-side cache: 12 sequences of 4000 tokens, 200 rows a key head, 54 us)
   const uint32_t groups = (uint32_t)a.n * a.h * a.splits;
   uint32_t group, tile;
   if (KW == 1) {
@@ -1247,16 +1248,17 @@ template <typename T, int DK, int NT, bool MASKED>
 void launch_tile_as(const AttnArgs& a, hipStream_t s) {
   const int64_t tiles = (a.G * a.Lq + 16 * NT - 1) / (16 * NT), groups = (int64_t)a.n * a.h * a.splits, units = groups * tiles;
   // a wave a unit where units fill the chip or keys are few, else a block a unit, whose waves have to meet at the end (wave / block,
-  // 0 .. keys tokens a sequence, 4 query heads a key head, bf16: DK = 128, 4096 units of 128 keys 26 / 51 us, of 1024 118 / 109, of
-  // 2048 214 / 190; DK = 256, where a block has its compute unit to itself, 1024 units of 128 keys 15 / 42, of 1024 60 / 79, of 4096
-  // 223 / 209; 132 rows a key head, DK = 64: 1536 units of 512 keys 37 / 46, of 2048 95 / 87)
+  // 0 .. keys tokens a sequence, 4 query heads a key head, bf16: DK = 128, 4096 units of 128 keys 26 / 53 us, of 1024 123 / 120, of
+  // 2048 230 / 203; DK = 256, where a block has its compute unit to itself, 1024 units of 128 keys 17 / 43, of 1024 68 / 82, 2048 units
+  // of 1024 126 / 153, of 4096 445 / 389; 132 rows a key head, DK = 64: 1520 units of 300 keys 20 / 27, of 2048 85 / 63)
   if (units >= (int64_t)a.chunk * (DK == 256 ? 1 : 3) || units + 8 * tiles > MAX_BLOCKS)
     hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 1, MASKED>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((kv8_attn_tile_kernel<T, DK, NT, 4, MASKED>), dim3((unsigned)((groups + 7) / 8 * 8 * tiles)), dim3(256), 0, s, a);
 }
-// masks are a variant of their own: looked up two groups ahead, a byte a lane and a ballot, they cost 2 to 5 % (23 sequences of 15 k tokens,
-// 99 rows a key head, DK = 256, all visible: 532 -> 269 us against eight byte loads a lane where they are needed)
+// masks are a variant of their own: looked up two groups ahead, a byte a lane and a ballot, they cost 7 to 16 % (23 sequences of 15 k
+// tokens, 99 rows a key head, DK = 256, all visible, with / without a mask: one key head bf16 135 / 126 us, two fp32 368 / 317; eight
+// byte loads a lane where they are needed took about twice the time)
 template <typename T, int DK, int NT>
 void launch_tile(const AttnArgs& a, hipStream_t s) {
   if (a.mask) launch_tile_as<T, DK, NT, true>(a, s);
@@ -1265,7 +1267,7 @@ void launch_tile(const AttnArgs& a, hipStream_t s) {
 template <typename T, int DK>
 void launch_dk(const AttnArgs& a, hipStream_t s) {
   // tiles of 16 rows a wave: what is unpacked once serves all of them, but two waves a SIMD have to stay (one query sequence of 512
-  // tokens, 32 heads, 8 key heads x 128 bf16, 4000 keys: 1 tile 99 us, 2 tiles 64 us = 525 TFLOP/s, 4 tiles, one wave a SIMD, 80 us).
+  // tokens, 32 heads, 8 key heads x 128 bf16, 4000 keys: 1 tile 116 us, 2 tiles 81 us = 414 TFLOP/s, 4 tiles, one wave a SIMD, 105 us).
   // A tile takes DK / 32 * pieces * 4 registers of queries, DK / 4 of sums and 8 of scores.
   constexpr int PER = DK / 32 * Pieces<T>::Q * 4 + DK / 4 + 8, MOST = 4 * PER <= 120 ? 4 : 2 * PER <= 120 ? 2 : 1;
   const int M = a.G * a.Lq;

@@ -115,7 +115,8 @@ class KV8Cache:
     def store(self, k, v, start=0, count=None, table=None):
         """Rows t < count[b] (None: all) of k, v (n, T, heads, dk) become tokens start[b] + t of sequence b.  `start` and
         `count` are numbers or int32 (n,) tensors on the device.  Overwriting from the middle of a sequence leaves what
-        stands behind it dead; no page may stand twice in the tables of one call."""
+        stands behind it dead; no page may be written for two sequences in one call.  Rows past a sequence's last page are dropped
+        (a number as `start` has to leave room for all T rows, unless `count` is a tensor), a negative start in a tensor stores nothing."""
         (k, *ks), (v, *vs) = _rows(k, "k"), _rows(v, "v")
         n, T = k.shape[:2]
         if v.shape != k.shape or v.dtype != k.dtype or tuple(k.shape[2:]) != (self.heads, self.dk):
